@@ -15,7 +15,7 @@ import sys
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRCS = [os.path.join(HERE, "csrc", n)
-        for n in ("kv_move.hip", "store_ring.cpp", "load_plan.cpp")]
+        for n in ("kv_move.hip", "kv_mx.hip", "store_ring.cpp", "load_plan.cpp")]
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "libdaser_kv.so")
 ABI_TEST_SRC = os.path.join(ROOT, "tests", "c", "abi_roundtrip.cpp")
@@ -89,7 +89,7 @@ def build_ring_sanitize(verbose: bool = False) -> None:
         return
     cmd = [clang, "-O1", "-g", "-fsanitize=address,undefined", "-fno-omit-frame-pointer",
            "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{INCLUDE}",
-           SRCS[1], RING_SAN_SRC, "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib",
+           SRCS[2], RING_SAN_SRC, "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib",
            "-o", RING_SAN_OUT + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)

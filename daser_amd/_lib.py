@@ -20,7 +20,7 @@ LIB_PATH = os.environ.get("DASER_KV_LIB") or os.path.join(
     os.path.dirname(os.path.abspath(__file__)), "libdaser_kv.so"
 )
 
-DSR_ABI_VERSION = 12
+DSR_ABI_VERSION = 13
 DSR_OK = 0
 DSR_ERR_ARG = -1
 DSR_ERR_ALIGN = -2
@@ -51,6 +51,9 @@ DSR_DTYPE_FP8_E5M2 = 3
 
 DSR_ROPE_NEOX = 0
 DSR_ROPE_GPTJ = 1
+
+DSR_MX_INT8 = 0
+DSR_MX_FP4 = 1
 
 DSR_SHARED_RECORDS = 1
 DSR_K_NHD, DSR_K_KX, DSR_K_HND = 0, 1, 2
@@ -105,6 +108,36 @@ class GatherArgs(ctypes.Structure):
                                       "num_heads", "reserved")]
 
 
+def _fields(spec: str) -> list:
+    kinds = {"p": _P, "q": _I64, "i": ctypes.c_int32, "f": ctypes.c_float}
+    return [(n, kinds[k]) for k, names in (part.split(":") for part in spec.split(";"))
+            for n in names.split()]
+
+
+class MxArgs(ctypes.Structure):
+    """dsr_mx_args."""
+
+    _fields_ = _fields("p:layer_base;q:kv_stride page_stride num_blocks;p:staging;"
+                       "q:staging_bytes layer_bytes;i:n_layers layer0 block_size num_heads "
+                       "head_dim dtype k_layout format")
+
+
+class MxRope(ctypes.Structure):
+    """dsr_mx_rope."""
+
+    _fields_ = _fields("p:cos_sin rope_idx layer_group;i:n_tables n_groups rot_dim style")
+
+
+class AttendArgs(ctypes.Structure):
+    """dsr_attend_args."""
+
+    _fields_ = _fields("p:q;q:q_row_stride q_head_stride;p:out lse prior_out prior_lse q_start "
+                       "page_start slot_offsets context limits rope_idx cos_sin staging;"
+                       "q:staging_bytes layer_bytes;p:workspace;q:workspace_bytes;f:scale;"
+                       "i:n_req n_q n_pages max_queries max_context q_heads kv_heads head_dim "
+                       "block_size layer n_tables rot_dim style dtype format")
+
+
 # Argument lists, one per exported entry point, in header order.
 _COPY_ARGS = [_P, _I, _I64, _I64, _I64, _I64, _P, _P, _I, _P, _I64, _I64, _I, _P]
 _SLOT_ARGS = [_P, _I, _I64, _I64, _I64, _I64, _I, _I64, _P, _P, _I, _P, _I64, _I64, _I, _P]
@@ -127,6 +160,13 @@ SIGNATURES = {
     "dsr_put": ([_P, _P, _I64, _P], _I),
     "dsr_delta_tables": ([_P, _I, _I, _P, _P], _I),
     "dsr_gather_layers": ([_P, _I, _I, _P], _I),
+    "dsr_mx_layer_bytes": ([_I, _I, _I, _I], _I64),
+    "dsr_gather_mx": ([_P, _I, _I, _P, _P, _I, _P], _I),
+    "dsr_scatter_mx": ([_P, _I, _I, _P, _P, _I, _P, _P], _I),
+    "dsr_gather_slots_mx": ([_P, _I, _I, _P, _P, _I, _P], _I),
+    "dsr_scatter_slots_mx": ([_P, _I, _I, _P, _P, _I, _P, _P], _I),
+    "dsr_attend_workspace": ([_P], _I64),
+    "dsr_attend_mx": ([_P, _P], _I),
     "dsr_ring_open": ([ctypes.c_char_p, _I64, _I, _I, ctypes.POINTER(_P)], _I),
     "dsr_ring_write": ([_P, _P, _I64, _I64, _P], _I),
     "dsr_ring_read": ([_P, _P, _I64, _I64, _P], _I),

@@ -1,6 +1,6 @@
 // kv_common.h -- constants, cache policies, the (page, layer) unit and its orders,
 // buffer descriptors and the copy engine shared by the kernels.
-// Part of libdaser_kv: included by kv_move.hip, one translation unit.
+// Part of libdaser_kv.
 
 #pragma once
 
@@ -10,6 +10,13 @@
 #include <atomic>
 
 #include "daser_kv.h"
+
+namespace dsr_detail {
+struct TuningKnobs {
+  std::atomic<int64_t> v[DSR_TUNE_COUNT_];
+};
+inline TuningKnobs g_tuning{};  // one for every translation unit
+}  // namespace dsr_detail
 
 namespace {
 
@@ -38,10 +45,7 @@ constexpr int kStoreNtSc = 19;
 // environment: a serving process gets the defaults unless its code asks.
 // Relaxed atomics, read once per call.
 enum RotKernelOverride { kRotAuto = 0, kRotPairs = 1 };
-struct TuningKnobs {
-  std::atomic<int64_t> v[DSR_TUNE_COUNT_];
-};
-TuningKnobs g_tuning{};
+using dsr_detail::g_tuning;
 inline int64_t tune(int knob) { return g_tuning.v[knob].load(std::memory_order_relaxed); }
 
 // Buffer descriptor word 3 for raw (untyped) dword access on CDNA3/4.

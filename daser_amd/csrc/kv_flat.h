@@ -1,5 +1,5 @@
 // kv_flat.h -- page gather and scatter as one flat run of 1 KiB pieces.
-// Part of libdaser_kv: included by kv_move.hip, one translation unit.
+// Part of libdaser_kv.
 //
 // A unit (page, layer) is cut into pieces of one wave instruction, 1 KiB of
 // its K run and the same 1 KiB of its V run, and each wave moves one piece: 2

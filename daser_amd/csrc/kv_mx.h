@@ -1,0 +1,399 @@
+// kv_mx.h -- quantised records (OCP microscaling formats): the elements' codecs and the
+// kernels that write records from the paged caches and read them back, by page and by
+// token.
+// Part of libdaser_kv: included by kv_mx.hip.
+//
+// A block of 32 elements of one (token, head) row is held as q_i 2^(s - 127). With a =
+// max |x_i|, s is the smallest code with a <= T 2^(s - 127), T the format's largest
+// value and half its last step (127.5 / 64, 7): a clipped element is then off by no more
+// than a rounded one may be. On N(0, 1) blocks e2m1 is off by 0.1118 sigma (rms) that
+// way, by 0.1149 under the rule floor(log2 a) and 0.1154 where nothing may clip.
+// Scaling by powers of two is exact, so there is one rounding, to the nearest code.
+//
+// Records hold a page head by head ([H][block_size][D]), whatever the cache's order: a
+// head's tokens lie in one run, which attention over records reads whole.
+
+#pragma once
+
+#include "kv_codec.h"
+#include "kv_flat.h"
+
+namespace {
+
+struct MxArgs {
+  const uint64_t* layer_base;
+  int64_t kv_stride, page_stride, num_blocks;
+  uint8_t* staging;
+  int64_t staging_bytes, layer_bytes, need;  // need: bytes of a layer in use
+  int64_t page_bytes;                        // of a cache page
+  int32_t layer0, first;  // table layers first ... are moved, record layers layer0 + l
+  int32_t vecs;           // 16-byte vectors (8 elements) of a page
+  int32_t codes, scales;  // section bytes of one half
+  int32_t heads, block;
+  FastDiv row_vecs, by_block, by_heads;  // vectors per row; block; heads
+};
+
+// A cache row's place in the record ([H][block]) and the other way round.
+struct MxRope {
+  const float2* cos_sin;
+  const int32_t* rope_idx;  // null: nothing is rotated
+  const int32_t* layer_group;
+  int32_t n_tables, n_groups;
+  int32_t rot_vecs, half_vecs;  // rotated vectors of a row; neox: to the partner
+};
+
+template <int FMT>
+__device__ __forceinline__ constexpr int mx_code_bytes() {  // of 8 elements
+  return FMT == DSR_MX_FP4 ? 4 : 8;
+}
+
+// E8M0 code of a block whose largest magnitude has these fp32 bits.
+template <int FMT>
+__device__ __forceinline__ uint32_t mx_scale_code(uint32_t bits) {
+  // bits + add carries into the exponent where the significand is past T's
+  constexpr uint32_t add = FMT == DSR_MX_FP4 ? 0x1fffffu : 0x00ffffu;
+  constexpr int sub = FMT == DSR_MX_FP4 ? 2 : 0;
+  const int s = (int)((bits + add) >> 23) - sub;
+  return bits >= 0x7f800000u ? 255u : (uint32_t)(s < 0 ? 0 : s);
+}
+
+// 2^(s - 127) for s < 255.
+__device__ __forceinline__ float mx_scale(uint32_t s) {
+  return __uint_as_float(s ? s << 23 : 0x00400000u);
+}
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+
+// fp32 bits of the largest magnitude of the 4 lanes' 8 elements each (one block);
+// 0x7F800000 and up: one of them is not finite.
+template <int DT>
+__device__ __forceinline__ uint32_t mx_block_max(u32x4 v) {
+  u16x2 m = __builtin_bit_cast(u16x2, v[0] & 0x7fff7fffu);
+#pragma unroll
+  for (int k = 1; k < 4; ++k)
+    m = __builtin_elementwise_max(m, __builtin_bit_cast(u16x2, v[k] & 0x7fff7fffu));
+  uint32_t a = m.x > m.y ? m.x : m.y;
+  const uint32_t b = (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0xb1, 0xf, 0xf, true);
+  a = a > b ? a : b;
+  const uint32_t c = (uint32_t)__builtin_amdgcn_mov_dpp((int)a, 0x4e, 0xf, 0xf, true);
+  a = a > c ? a : c;
+  if (DT == DSR_DTYPE_BF16) return a << 16;
+  return a >= 0x7c00u ? 0x7f800000u : __float_as_uint(fp16_to_f32(a));
+}
+
+// 8 elements of a cache vector as codes under scale code s.
+template <int FMT, int DT>
+__device__ __forceinline__ uint2 mx_encode(u32x4 v, uint32_t s) {
+  uint2 o{0u, 0u};
+  if (FMT == DSR_MX_FP4) {
+    const float scale = mx_scale(s);
+// (the pair in a variable of its own: a bit cast of a vector's element takes the first)
+#define DSR_FP4(K)                                                                             \
+  {                                                                                            \
+    const uint32_t w = v[K];                                                                   \
+    if (DT == DSR_DTYPE_BF16)                                                                  \
+      o.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_bf16(o.x, __builtin_bit_cast(bf16x2, w), scale, \
+                                                      K);                                      \
+    else                                                                                       \
+      o.x = __builtin_amdgcn_cvt_scalef32_pk_fp4_f16(o.x, __builtin_bit_cast(f16x2, w), scale, K); \
+  }
+    DSR_FP4(0)
+    DSR_FP4(1)
+    DSR_FP4(2)
+    DSR_FP4(3)
+#undef DSR_FP4
+  } else {
+    float x[8];
+    Codec<DT>::decode(v, x);
+    uint32_t b[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float y = __builtin_ldexpf(x[e], 133 - (int)s);
+      y = __builtin_fminf(__builtin_fmaxf(y, -127.0f), 127.0f);
+      b[e] = __float_as_uint(y + 12582912.0f);  // 1.5 * 2^23: the low byte is rne(y)
+    }
+    const uint32_t l = __builtin_amdgcn_perm(b[1], b[0], 0x0c0c0400u);
+    const uint32_t h = __builtin_amdgcn_perm(b[3], b[2], 0x04000c0cu);
+    o.x = l | h;
+    o.y = __builtin_amdgcn_perm(b[5], b[4], 0x0c0c0400u) |
+          __builtin_amdgcn_perm(b[7], b[6], 0x04000c0cu);
+  }
+  if (s == 255u) o = uint2{0u, 0u};
+  return o;
+}
+
+// Values of 8 codes under scale code s, NaN under 255.
+template <int FMT>
+__device__ __forceinline__ void mx_decode(uint2 c, uint32_t s, float* x) {
+  if (FMT == DSR_MX_FP4) {
+    const float scale = mx_scale(s);
+    f32x2 f[4];
+    f[0] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, scale, 0);
+    f[1] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, scale, 1);
+    f[2] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, scale, 2);
+    f[3] = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, scale, 3);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      x[2 * k] = f[k].x;
+      x[2 * k + 1] = f[k].y;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const uint32_t w = e < 4 ? c.x : c.y;
+      x[e] = __builtin_ldexpf((float)(int8_t)(w >> (8 * (e & 3))), (int)s - 133);
+    }
+  }
+  if (s == 255u) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(0x7fc00000u);
+  }
+}
+
+// 8 values as a cache vector: saturated to the type's largest, NaN kept.
+template <int DT>
+__device__ __forceinline__ u32x4 mx_store_vec(float* y) {
+  const float top = DT == DSR_DTYPE_BF16 ? __uint_as_float(0x7f7f0000u) : 65504.0f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    y[e] = y[e] > top ? top : y[e];
+    y[e] = y[e] < -top ? -top : y[e];
+  }
+  u32x4 v;
+  if constexpr (DT == DSR_DTYPE_BF16) {
+    if (Codec<DT>::encode_quick(y, &v)) v = Codec<DT>::encode(y);
+  } else {
+    v = Codec<DT>::encode(y);
+  }
+  return v;
+}
+
+// One half (K or V) of a record's layer.
+struct MxHalf {
+  const uint8_t* codes;
+  const uint8_t* scales;
+};
+__device__ __forceinline__ MxHalf mx_half(const MxArgs& a, const uint8_t* rec, int half) {
+  return {rec + (int64_t)half * a.codes, rec + 2 * (int64_t)a.codes + (int64_t)half * a.scales};
+}
+
+template <int FMT>
+__device__ __forceinline__ uint2 mx_load_codes(const MxHalf& h, int vec) {
+  if (FMT == DSR_MX_FP4) return uint2{reinterpret_cast<const uint32_t*>(h.codes)[vec], 0u};
+  return reinterpret_cast<const uint2*>(h.codes)[vec];
+}
+
+// Cache vector of record vector `rv`, whose row in the record is that of (t, h), read
+// and, for K, rotated by table `cs` (null: not); c: the vector's column in its row.
+template <int FMT, int DT, int STYLE>
+__device__ __forceinline__ u32x4 mx_read_vec(const MxHalf& half, int rv, int c, const MxRope& r,
+                                             const float2* cs) {
+  float x[8];
+  mx_decode<FMT>(mx_load_codes<FMT>(half, rv), half.scales[rv >> 2], x);
+  if (cs && c < r.rot_vecs) {
+    float t[8];
+    if (STYLE == DSR_ROPE_NEOX) {
+      const bool lower = c < r.half_vecs;
+      const int pv = lower ? rv + r.half_vecs : rv - r.half_vecs;
+      mx_decode<FMT>(mx_load_codes<FMT>(half, pv), half.scales[pv >> 2], t);
+      const float2* p = cs + (lower ? c : c - r.half_vecs) * 8;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 w = p[e];
+        const float ps = t[e] * w.y;
+        x[e] = __builtin_fmaf(x[e], w.x, lower ? -ps : ps);
+      }
+    } else {
+      const float2* p = cs + c * 4;
+#pragma unroll
+      for (int e = 0; e < 8; e += 2) {
+        const float2 w = p[e / 2];
+        const float u = x[e], v = x[e + 1];
+        const float us = u * w.y, vs = v * w.y;
+        x[e] = __builtin_fmaf(u, w.x, -vs);
+        x[e + 1] = __builtin_fmaf(v, w.x, us);
+      }
+    }
+  }
+  return mx_store_vec<DT>(x);
+}
+
+// Table of entry p in record layer l, or null.
+__device__ __forceinline__ const float2* mx_table(const MxRope& r, int64_t p, int l) {
+  if (!r.rope_idx) return nullptr;
+  int t = r.rope_idx[p];
+  if (t < 0 || t >= r.n_tables) return nullptr;
+  if (r.layer_group) {
+    const int g = r.layer_group[l];
+    if (g < 0 || g >= r.n_groups) return nullptr;
+    t += g * r.n_tables;
+  }
+  return r.cos_sin + (int64_t)t * (r.rot_vecs * 4);
+}
+
+struct MxPos {
+  uint8_t* cache;
+  uint8_t* rec;
+  uint32_t page;
+  int layer;  // of the record
+  int part;
+};
+
+// This wave's piece, as flat_pos finds it; false past the launch's end and for entries
+// out of bounds.
+template <bool kPageMajor>
+__device__ __forceinline__ bool mx_pos(const MxArgs& a, const FlatMap& m, const int32_t* page_ids,
+                                       const int64_t* slot_offsets, MxPos* o) {
+  const uint32_t w = flat_wave(m);
+  if (w >= m.n_waves) return false;
+  const uint32_t g = m.wave0 + w;
+  const uint32_t q = div_by(g, m.per_unit);
+  o->part = (int)(g - q * m.per_unit.d);
+  const uint32_t v = m.unit0 + q;
+  const uint32_t hi = div_by(v, m.minor);
+  const uint32_t lo = v - hi * m.minor.d;
+  const uint32_t p = kPageMajor ? hi : lo;
+  const int l = a.first + (int)(kPageMajor ? lo : hi);
+  const int64_t blk = page_ids[p];
+  const int64_t rec = slot_offsets[p], off = rec + (int64_t)(a.layer0 + l) * a.layer_bytes;
+  if (blk < 0 || blk >= a.num_blocks) return false;
+  if (rec < 0 || off + a.need > a.staging_bytes) return false;
+  o->cache = reinterpret_cast<uint8_t*>(a.layer_base[l]) + blk * a.page_stride;
+  o->rec = a.staging + off;
+  o->page = p;
+  o->layer = a.layer0 + l;
+  return true;
+}
+
+// Pages -> records. A wave takes 64 vectors of K and of V in the record's order.
+template <int FMT, int DT, bool HND>
+__global__ __launch_bounds__(kThreads) void kv_mx_gather_kernel(MxArgs a, const int32_t* page_ids,
+                                                                const int64_t* slot_offsets,
+                                                                FlatMap m) {
+  MxPos u;
+  if (!mx_pos<true>(a, m, page_ids, slot_offsets, &u)) return;
+  const int rv = u.part * kWave + (int)threadIdx.x % kWave;
+  const bool in = rv < a.vecs;
+  int cv = rv;
+  if (!HND) {
+    const int row = (int)div_by((uint32_t)rv, a.row_vecs);
+    const int c = rv - row * (int)a.row_vecs.d;
+    const int h = (int)div_by((uint32_t)row, a.by_block);
+    const int t = row - h * a.block;
+    cv = (t * a.heads + h) * (int)a.row_vecs.d + c;
+  }
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const rsrc_t r = make_rsrc(u.cache + (half ? a.kv_stride : 0), a.page_bytes);
+    const u32x4 v = bload(r, in ? cv << 4 : (int)a.page_bytes);
+    const uint32_t s = mx_scale_code<FMT>(mx_block_max<DT>(v));
+    const uint2 q = mx_encode<FMT, DT>(v, s);
+    if (!in) continue;
+    const MxHalf o = mx_half(a, u.rec, half);
+    if (FMT == DSR_MX_FP4)
+      reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(o.codes))[rv] = q.x;
+    else
+      reinterpret_cast<uint2*>(const_cast<uint8_t*>(o.codes))[rv] = q;
+    if ((rv & 3) == 0) const_cast<uint8_t*>(o.scales)[rv >> 2] = (uint8_t)s;
+  }
+}
+
+// Records -> pages. A wave takes 64 vectors of K and of V in the cache page's order.
+template <int FMT, int DT, bool HND, int STYLE>
+__global__ __launch_bounds__(kThreads) void kv_mx_scatter_kernel(MxArgs a, MxRope r,
+                                                                 const int32_t* page_ids,
+                                                                 const int64_t* slot_offsets,
+                                                                 FlatMap m) {
+  MxPos u;
+  if (!mx_pos<false>(a, m, page_ids, slot_offsets, &u)) return;
+  const int cv = u.part * kWave + (int)threadIdx.x % kWave;
+  if (cv >= a.vecs) return;
+  const int row = (int)div_by((uint32_t)cv, a.row_vecs);
+  const int c = cv - row * (int)a.row_vecs.d;
+  int rv = cv;
+  if (!HND) {
+    const int t = (int)div_by((uint32_t)row, a.by_heads);
+    const int h = row - t * a.heads;
+    rv = (h * a.block + t) * (int)a.row_vecs.d + c;
+  }
+  const float2* cs = mx_table(r, u.page, u.layer);
+  const u32x4 k = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 0), rv, c, r, cs);
+  const u32x4 v = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 1), rv, c, r, nullptr);
+  *reinterpret_cast<u32x4*>(u.cache + ((int64_t)cv << 4)) = k;
+  *reinterpret_cast<u32x4*>(u.cache + a.kv_stride + ((int64_t)cv << 4)) = v;
+}
+
+// The token form: lane = one vector of one token's K and V rows, layer blockIdx.y.
+struct MxToken {
+  uint8_t* cache;
+  uint8_t* rec;
+  int cv, rv, c;  // vectors in the cache page and in the record; column in the row
+  int64_t token;
+};
+template <bool HND>
+__device__ __forceinline__ bool mx_token(const MxArgs& a, const int64_t* slots,
+                                         const int64_t* rows, uint32_t n, FastDiv per_token,
+                                         int l, MxToken* o) {
+  const uint32_t i = blockIdx.x * kThreads + threadIdx.x;
+  const uint32_t t = div_by(i, per_token);
+  if (t >= n) return false;
+  const uint32_t v = i - t * per_token.d;
+  const int h = (int)div_by(v, a.row_vecs);
+  o->c = (int)(v - (uint32_t)h * a.row_vecs.d);
+  const int64_t slot = slots[t], row = rows[t];
+  if (slot < 0 || row < 0) return false;
+  const int64_t blk = slot / a.block, off = row / a.block;
+  const int ct = (int)(slot - blk * a.block), rt = (int)(row - off * a.block);
+  if (blk >= a.num_blocks || (off & 15)) return false;
+  const int64_t at = off + (int64_t)(a.layer0 + l) * a.layer_bytes;
+  if (at + a.need > a.staging_bytes) return false;
+  o->cache = reinterpret_cast<uint8_t*>(a.layer_base[l]) + blk * a.page_stride;
+  o->rec = a.staging + at;
+  o->cv = (HND ? h * a.block + ct : ct * a.heads + h) * (int)a.row_vecs.d + o->c;
+  o->rv = (h * a.block + rt) * (int)a.row_vecs.d + o->c;
+  o->token = t;
+  return true;
+}
+
+template <int FMT, int DT, bool HND>
+__global__ __launch_bounds__(kThreads) void kv_mx_gather_slots_kernel(MxArgs a,
+                                                                      const int64_t* slots,
+                                                                      const int64_t* rows,
+                                                                      uint32_t n,
+                                                                      FastDiv per_token) {
+  MxToken u;
+  // the 4 lanes of a block belong to one token and leave together
+  if (!mx_token<HND>(a, slots, rows, n, per_token, a.first + (int)blockIdx.y, &u)) return;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const u32x4 v = *reinterpret_cast<const u32x4*>(u.cache + (half ? a.kv_stride : 0) +
+                                                    ((int64_t)u.cv << 4));
+    const uint32_t s = mx_scale_code<FMT>(mx_block_max<DT>(v));
+    const uint2 q = mx_encode<FMT, DT>(v, s);
+    const MxHalf o = mx_half(a, u.rec, half);
+    if (FMT == DSR_MX_FP4)
+      reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(o.codes))[u.rv] = q.x;
+    else
+      reinterpret_cast<uint2*>(const_cast<uint8_t*>(o.codes))[u.rv] = q;
+    if ((u.rv & 3) == 0) const_cast<uint8_t*>(o.scales)[u.rv >> 2] = (uint8_t)s;
+  }
+}
+
+template <int FMT, int DT, bool HND, int STYLE>
+__global__ __launch_bounds__(kThreads) void kv_mx_scatter_slots_kernel(MxArgs a, MxRope r,
+                                                                       const int64_t* slots,
+                                                                       const int64_t* rows,
+                                                                       uint32_t n,
+                                                                       FastDiv per_token) {
+  MxToken u;
+  const int l = a.first + (int)blockIdx.y;
+  if (!mx_token<HND>(a, slots, rows, n, per_token, l, &u)) return;
+  const float2* cs = mx_table(r, u.token, a.layer0 + l);
+  const u32x4 k = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 0), u.rv, u.c, r, cs);
+  const u32x4 v = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 1), u.rv, u.c, r, nullptr);
+  *reinterpret_cast<u32x4*>(u.cache + ((int64_t)u.cv << 4)) = k;
+  *reinterpret_cast<u32x4*>(u.cache + a.kv_stride + ((int64_t)u.cv << 4)) = v;
+}
+
+}  // namespace

@@ -1,0 +1,307 @@
+// kv_mx.hip -- launch policy and C ABI of the quantised records (kv_mx.h) and of the
+// attention over them (kv_attend.h).
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "kv_attend.h"
+#include "kv_launch.h"
+
+namespace {
+
+int64_t pad16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Section bytes of one half; false for geometries that the format does not take.
+bool mx_sections(int format, int block, int heads, int dim, int64_t* codes, int64_t* scales) {
+  if (block <= 0 || heads <= 0 || dim <= 0 || dim % 32) return false;
+  const __int128 elems = (__int128)block * heads * dim;
+  if (elems * 2 > 0x7fffffffLL) return false;  // one buffer descriptor per cache page
+  *codes = pad16((int64_t)elems / (format == DSR_MX_FP4 ? 2 : 1));
+  *scales = pad16((int64_t)elems / 32);
+  return true;
+}
+
+// Checks a call's caches, records and layers; fills the kernels' arguments.
+int mx_args(const dsr_mx_args* in, int first, int count, const void* t1, const void* t2, int n,
+            MxArgs* a) {
+  if (!in || n < 0 || first < 0 || count < 0 || in->n_layers < 0 || in->layer0 < 0 ||
+      first > in->n_layers - count || in->num_blocks < 0 || in->staging_bytes < 0)
+    return DSR_ERR_ARG;
+  if (in->format != DSR_MX_INT8 && in->format != DSR_MX_FP4) return DSR_ERR_ARG;
+  if (in->dtype != DSR_DTYPE_BF16 && in->dtype != DSR_DTYPE_FP16) return DSR_ERR_ARG;
+  if (in->k_layout == DSR_K_KX) return DSR_ERR_SHAPE;
+  if (in->k_layout != DSR_K_NHD && in->k_layout != DSR_K_HND) return DSR_ERR_ARG;
+  int64_t codes, scales;
+  if (!mx_sections(in->format, in->block_size, in->num_heads, in->head_dim, &codes, &scales) ||
+      in->layer_bytes < 2 * (codes + scales))
+    return DSR_ERR_SHAPE;
+  if (n == 0 || count == 0) return DSR_OK;
+  if (!in->layer_base || !in->staging || !t1 || !t2) return DSR_ERR_ARG;
+  if (!aligned16(in->kv_stride) || !aligned16(in->page_stride) || !aligned16(in->layer_bytes) ||
+      !aligned16p(in->staging))
+    return DSR_ERR_ALIGN;
+  *a = MxArgs{};
+  a->layer_base = in->layer_base;
+  a->kv_stride = in->kv_stride;
+  a->page_stride = in->page_stride;
+  a->num_blocks = in->num_blocks;
+  a->staging = static_cast<uint8_t*>(in->staging);
+  a->staging_bytes = in->staging_bytes;
+  a->layer_bytes = in->layer_bytes;
+  a->need = 2 * (codes + scales);
+  a->page_bytes = 2LL * in->block_size * in->num_heads * in->head_dim;
+  a->layer0 = in->layer0;
+  a->first = first;
+  a->vecs = (int)(a->page_bytes >> 4);
+  a->codes = (int)codes;
+  a->scales = (int)scales;
+  a->heads = in->num_heads;
+  a->block = in->block_size;
+  a->row_vecs = fast_div((uint32_t)in->head_dim / 8);
+  a->by_block = fast_div((uint32_t)in->block_size);
+  a->by_heads = fast_div((uint32_t)in->num_heads);
+  return DSR_OK;
+}
+
+int mx_rope(const dsr_mx_args* in, const dsr_mx_rope* rope, MxRope* r) {
+  *r = MxRope{};
+  if (!rope) return DSR_OK;
+  if (rope->style != DSR_ROPE_NEOX && rope->style != DSR_ROPE_GPTJ) return DSR_ERR_ARG;
+  if (rope->n_tables < 0 || (rope->layer_group && rope->n_groups < 1)) return DSR_ERR_ARG;
+  if (!rope->rope_idx || (rope->n_tables > 0 && !rope->cos_sin)) return DSR_ERR_ARG;
+  const int rd = rope->rot_dim;
+  if (rd <= 0 || rd > in->head_dim || rd % (rope->style == DSR_ROPE_NEOX ? 16 : 8))
+    return DSR_ERR_SHAPE;
+  r->cos_sin = reinterpret_cast<const float2*>(rope->cos_sin);
+  r->rope_idx = rope->rope_idx;
+  r->layer_group = rope->layer_group;
+  r->n_tables = rope->n_tables;
+  r->n_groups = rope->n_groups;
+  r->rot_vecs = rd / 8;
+  r->half_vecs = rope->style == DSR_ROPE_NEOX ? rd / 16 : 0;
+  return DSR_OK;
+}
+
+// f<FMT, DT, HND>() of the call's format, type and layout.
+template <class F>
+void mx_dispatch(const dsr_mx_args* in, F f) {
+#define DSR_MX_HND(FMT, DT)                                                \
+  if (in->k_layout == DSR_K_HND) f.template operator()<FMT, DT, true>();   \
+  else f.template operator()<FMT, DT, false>()
+#define DSR_MX_DT(FMT)                                                 \
+  if (in->dtype == DSR_DTYPE_BF16) { DSR_MX_HND(FMT, DSR_DTYPE_BF16); } \
+  else { DSR_MX_HND(FMT, DSR_DTYPE_FP16); }
+  if (in->format == DSR_MX_FP4) {
+    DSR_MX_DT(DSR_MX_FP4)
+  } else {
+    DSR_MX_DT(DSR_MX_INT8)
+  }
+#undef DSR_MX_DT
+#undef DSR_MX_HND
+}
+
+struct GatherPages {
+  const MxArgs& a;
+  const int32_t* ids;
+  const int64_t* offs;
+  const FlatMap& m;
+  unsigned grid;
+  hipStream_t s;
+  template <int FMT, int DT, bool HND>
+  void operator()() const {
+    kv_mx_gather_kernel<FMT, DT, HND><<<grid, kThreads, 0, s>>>(a, ids, offs, m);
+  }
+};
+struct ScatterPages {
+  const MxArgs& a;
+  const MxRope& r;
+  int style;
+  const int32_t* ids;
+  const int64_t* offs;
+  const FlatMap& m;
+  unsigned grid;
+  hipStream_t s;
+  template <int FMT, int DT, bool HND>
+  void operator()() const {
+    if (style == DSR_ROPE_NEOX)
+      kv_mx_scatter_kernel<FMT, DT, HND, DSR_ROPE_NEOX><<<grid, kThreads, 0, s>>>(a, r, ids, offs, m);
+    else
+      kv_mx_scatter_kernel<FMT, DT, HND, DSR_ROPE_GPTJ><<<grid, kThreads, 0, s>>>(a, r, ids, offs, m);
+  }
+};
+struct Tokens {
+  const MxArgs& a;
+  const MxRope* r;  // null: gather
+  int style;
+  const int64_t* slots;
+  const int64_t* rows;
+  uint32_t n;
+  FastDiv per;
+  dim3 grid;
+  hipStream_t s;
+  template <int FMT, int DT, bool HND>
+  void operator()() const {
+    if (!r)
+      kv_mx_gather_slots_kernel<FMT, DT, HND><<<grid, kThreads, 0, s>>>(a, slots, rows, n, per);
+    else if (style == DSR_ROPE_NEOX)
+      kv_mx_scatter_slots_kernel<FMT, DT, HND, DSR_ROPE_NEOX>
+          <<<grid, kThreads, 0, s>>>(a, *r, slots, rows, n, per);
+    else
+      kv_mx_scatter_slots_kernel<FMT, DT, HND, DSR_ROPE_GPTJ>
+          <<<grid, kThreads, 0, s>>>(a, *r, slots, rows, n, per);
+  }
+};
+
+// Token-form launches: tokens in ranges whose vectors, and layers in ranges that, one
+// grid holds.
+int launch_tokens(const dsr_mx_args* in, MxArgs a, const MxRope* rope, int style, int count,
+                  const int64_t* slots, const int64_t* rows, int n, hipStream_t s) {
+  const int64_t vecs = (int64_t)in->num_heads * in->head_dim / 8;  // of one token
+  const int64_t wgs = max_wg_per_launch();
+  const int layers = (int)(wgs < 65535 ? wgs : 65535);
+  int64_t per = wgs / (count < layers ? count : layers) * kThreads / vecs;
+  if (per < 1) per = 1;
+  MxRope r = rope ? *rope : MxRope{};
+  for (int l0 = 0; l0 < count; l0 += layers) {
+    const int nl = count - l0 < layers ? count - l0 : layers;
+    MxArgs b = a;
+    b.first += l0;
+    for (int64_t t0 = 0; t0 < n; t0 += per) {
+      const int64_t nt = n - t0 < per ? n - t0 : per;
+      const dim3 grid((unsigned)((nt * vecs + kThreads - 1) / kThreads), (unsigned)nl);
+      if (rope) r.rope_idx = rope->rope_idx ? rope->rope_idx + t0 : nullptr;
+      mx_dispatch(in, Tokens{b, rope ? &r : nullptr, style, slots + t0, rows + t0, (uint32_t)nt,
+                             fast_div((uint32_t)vecs), grid, s});
+      const int rc = (int)hipGetLastError();
+      if (rc != 0) return rc;
+    }
+  }
+  return DSR_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int64_t dsr_mx_layer_bytes(int format, int block_size, int num_heads, int head_dim) {
+  if (format != DSR_MX_INT8 && format != DSR_MX_FP4) return DSR_ERR_ARG;
+  int64_t codes, scales;
+  if (!mx_sections(format, block_size, num_heads, head_dim, &codes, &scales)) return DSR_ERR_SHAPE;
+  return 2 * (codes + scales);
+}
+
+int dsr_gather_mx(const dsr_mx_args* args, int first, int count, const int32_t* page_ids,
+                  const int64_t* slot_offsets, int n_pages, dsr_stream_t stream) {
+  MxArgs a;
+  const int rc = mx_args(args, first, count, page_ids, slot_offsets, n_pages, &a);
+  if (rc != DSR_OK || n_pages == 0 || count == 0) return rc;
+  if ((int64_t)n_pages * count > 0x7fffffffLL) return DSR_ERR_ARG;
+  return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, count, 0,
+                     [&](const FlatMap& m, unsigned grid) {
+    mx_dispatch(args, GatherPages{a, page_ids, slot_offsets, m, grid, (hipStream_t)stream});
+  });
+}
+
+int dsr_scatter_mx(const dsr_mx_args* args, int first, int count, const int32_t* page_ids,
+                   const int64_t* slot_offsets, int n_pages, const dsr_mx_rope* rope,
+                   dsr_stream_t stream) {
+  MxArgs a;
+  MxRope r;
+  int rc = mx_args(args, first, count, page_ids, slot_offsets, n_pages, &a);
+  if (rc != DSR_OK || n_pages == 0 || count == 0) return rc;
+  if ((rc = mx_rope(args, rope, &r)) != DSR_OK) return rc;
+  if ((int64_t)n_pages * count > 0x7fffffffLL) return DSR_ERR_ARG;
+  return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, n_pages, 0,
+                     [&](const FlatMap& m, unsigned grid) {
+    mx_dispatch(args, ScatterPages{a, r, rope ? rope->style : DSR_ROPE_NEOX, page_ids,
+                                   slot_offsets, m, grid, (hipStream_t)stream});
+  });
+}
+
+int dsr_gather_slots_mx(const dsr_mx_args* args, int first, int count,
+                        const int64_t* slot_mapping, const int64_t* record_rows, int n_tokens,
+                        dsr_stream_t stream) {
+  MxArgs a;
+  const int rc = mx_args(args, first, count, slot_mapping, record_rows, n_tokens, &a);
+  if (rc != DSR_OK || n_tokens == 0 || count == 0) return rc;
+  return launch_tokens(args, a, nullptr, 0, count, slot_mapping, record_rows, n_tokens,
+                       (hipStream_t)stream);
+}
+
+int dsr_scatter_slots_mx(const dsr_mx_args* args, int first, int count,
+                         const int64_t* slot_mapping, const int64_t* record_rows, int n_tokens,
+                         const dsr_mx_rope* rope, dsr_stream_t stream) {
+  MxArgs a;
+  MxRope r;
+  int rc = mx_args(args, first, count, slot_mapping, record_rows, n_tokens, &a);
+  if (rc != DSR_OK || n_tokens == 0 || count == 0) return rc;
+  if ((rc = mx_rope(args, rope, &r)) != DSR_OK) return rc;
+  return launch_tokens(args, a, &r, rope ? rope->style : DSR_ROPE_NEOX, count, slot_mapping,
+                       record_rows, n_tokens, (hipStream_t)stream);
+}
+
+int64_t dsr_attend_workspace(const dsr_attend_args* args) {
+  if (!args) return DSR_ERR_ARG;
+  return 0;
+}
+
+int dsr_attend_mx(const dsr_attend_args* args, dsr_stream_t stream) {
+  if (!args) return DSR_ERR_ARG;
+  const dsr_attend_args& a = *args;
+  if (a.n_req < 0 || a.n_q < 0 || a.n_pages < 0 || a.max_queries < 0 || a.max_context < 0 ||
+      a.layer < 0 || a.staging_bytes < 0 || a.n_tables < 0 || a.workspace_bytes < 0)
+    return DSR_ERR_ARG;
+  if (a.format != DSR_MX_INT8 && a.format != DSR_MX_FP4) return DSR_ERR_ARG;
+  if (a.dtype != DSR_DTYPE_BF16 && a.dtype != DSR_DTYPE_FP16) return DSR_ERR_ARG;
+  int64_t codes, scales;
+  if (!mx_sections(a.format, a.block_size, a.kv_heads, a.head_dim, &codes, &scales) ||
+      a.layer_bytes < 2 * (codes + scales) || a.block_size % 16 || a.q_heads <= 0 ||
+      a.q_heads % a.kv_heads || a.q_heads > 65535)
+    return DSR_ERR_SHAPE;
+  const int d = a.head_dim;
+  if (d != 32 && d != 64 && d != 96 && d != 128 && d != 256) return DSR_ERR_SHAPE;
+  if (a.rope_idx) {
+    if (a.style != DSR_ROPE_NEOX && a.style != DSR_ROPE_GPTJ) return DSR_ERR_ARG;
+    if (a.n_tables > 0 && !a.cos_sin) return DSR_ERR_ARG;
+    if (a.rot_dim <= 0 || a.rot_dim > d || a.rot_dim % (a.style == DSR_ROPE_NEOX ? 16 : 8))
+      return DSR_ERR_SHAPE;
+  }
+  if (a.n_req == 0 || a.n_q == 0) return DSR_OK;
+  if (!a.q || !a.out || !a.lse || !a.q_start || !a.page_start || !a.context ||
+      (a.n_pages > 0 && (!a.slot_offsets || !a.staging)) || !a.prior_out != !a.prior_lse)
+    return DSR_ERR_ARG;
+  if (!aligned16(a.q_row_stride) || !aligned16(a.q_head_stride) || !aligned16p(a.q) ||
+      !aligned16p(a.out) || !aligned16p(a.prior_out) || !aligned16p(a.staging) ||
+      !aligned16(a.layer_bytes) || !aligned16p(a.workspace))
+    return DSR_ERR_ALIGN;
+  AttendArgs g{a, (int)codes, (int)scales, 2 * (codes + scales)};
+  const int64_t most = max_wg_per_launch();
+  hipStream_t s = (hipStream_t)stream;
+  for (int r0 = 0; r0 < a.n_req; r0 += 65535) {
+    const int n = a.n_req - r0 < 65535 ? a.n_req - r0 : 65535;
+    int64_t x = a.max_queries < 1 ? 1 : a.max_queries;
+    const int64_t room = most / a.q_heads / n;
+    if (x > room) x = room < 1 ? 1 : room;
+    const dim3 grid((unsigned)x, (unsigned)a.q_heads, (unsigned)n);
+    AttendArgs b = g;
+    b.a.q_start += r0;
+    b.a.page_start += r0;
+    b.a.context += r0;
+    if (a.format == DSR_MX_FP4) {
+      if (a.dtype == DSR_DTYPE_BF16)
+        kv_mx_attend_simple_kernel<DSR_MX_FP4, DSR_DTYPE_BF16><<<grid, kWave, 0, s>>>(b);
+      else
+        kv_mx_attend_simple_kernel<DSR_MX_FP4, DSR_DTYPE_FP16><<<grid, kWave, 0, s>>>(b);
+    } else {
+      if (a.dtype == DSR_DTYPE_BF16)
+        kv_mx_attend_simple_kernel<DSR_MX_INT8, DSR_DTYPE_BF16><<<grid, kWave, 0, s>>>(b);
+      else
+        kv_mx_attend_simple_kernel<DSR_MX_INT8, DSR_DTYPE_FP16><<<grid, kWave, 0, s>>>(b);
+    }
+    const int rc = (int)hipGetLastError();
+    if (rc != 0) return rc;
+  }
+  return DSR_OK;
+}
+
+}  // extern "C"

@@ -52,9 +52,9 @@ typedef struct ihipStream_t* dsr_stream_t; /* == hipStream_t */
  * dsr_set_tuning, 7 dsr_scatter_ex, 8 dsr_scatter_slots_rerotate, 9
  * DSR_RING_MMAP and dsr_ring_is_mapped, 10 dsr_scatter_rerotate_static, 11
  * dsr_scatter_fanout, 12 the host-table planners (dsr_plan_*), dsr_put,
- * dsr_delta_tables and dsr_gather_layers. Callers check dsr_abi_version()
- * against it. */
-#define DSR_ABI_VERSION 12
+ * dsr_delta_tables and dsr_gather_layers, 13 the quantised records (dsr_*_mx).
+ * Callers check dsr_abi_version() against it. */
+#define DSR_ABI_VERSION 13
 
 /*
  * Kernel choice and launch shape follow from the geometry. dsr_set_tuning()
@@ -570,6 +570,131 @@ typedef struct {
   int32_t n_layers, layer0, n_pages, block_size, num_heads, reserved;
 } dsr_gather_args;
 int dsr_gather_layers(const dsr_gather_args* args, int first, int count, dsr_stream_t stream);
+
+/*
+ * Quantised records: slot records in the OCP microscaling (MX) formats, written
+ * from 16-bit caches, read back into them, and attended in place. The reference
+ * stores every record in the cache's own type (daser/connector/
+ * daser_connector.py:625-632); these replace the same loops (:536-551 the load)
+ * where a store is to hold 1.94 (DSR_MX_INT8) or 3.76 times (DSR_MX_FP4) as much.
+ *
+ * Format. 32 consecutive elements of one token's head form a block with one scale
+ * 2^(s - 127), s a byte (E8M0). Elements: DSR_MX_INT8 two's complement q / 64;
+ * DSR_MX_FP4 e2m1 (0 .5 1 1.5 2 3 4 6 and a sign), two to a byte, the first in the
+ * low half. A layer of a record is
+ *     K codes [H][block_size][D] | V codes | K scales [H][block_size][D / 32] | V scales
+ * each section rounded up to 16 bytes, dsr_mx_layer_bytes() in all, in every cache
+ * layout: the record of (page p, layer l) starts at staging + slot_offsets[p] +
+ * (layer0 + l) * layer_bytes. A negative slot offset is skipped in every layer.
+ *
+ * Writing: s is the smallest scale under which the block's largest magnitude is at
+ * most half a step past the format's largest (127.5 / 64, 7), each element is
+ * rounded to nearest even and saturated. A block with a NaN or an infinity gets
+ * s = 255. Reading: q * 2^(s - 127) rounded to the cache's type (exact in bf16, and
+ * in fp16 but for subnormals) and saturated to its largest finite value; s = 255
+ * reads as NaN (0x7FC0, 0x7E00).
+ */
+#define DSR_MX_INT8 0
+#define DSR_MX_FP4 1
+
+/* The caches and records of a call. Layouts and strides as above; a cache of
+ * DSR_K_KX is refused (DSR_ERR_SHAPE). head_dim must be a multiple of 32, a
+ * page's bytes fit 31 bits, layer_bytes at least dsr_mx_layer_bytes(). */
+typedef struct {
+  const uint64_t* layer_base; /* [device] */
+  int64_t kv_stride, page_stride, num_blocks;
+  void* staging;
+  int64_t staging_bytes, layer_bytes;
+  int32_t n_layers, layer0;
+  int32_t block_size, num_heads, head_dim;
+  int32_t dtype;    /* DSR_DTYPE_BF16 or DSR_DTYPE_FP16 */
+  int32_t k_layout; /* DSR_K_NHD or DSR_K_HND */
+  int32_t format;   /* DSR_MX_* */
+} dsr_mx_args;
+
+/* The rotation of a load's K, as dsr_scatter_rerotate's arguments (rope_idx per page
+ * or per token). rot_dim must be a multiple of 16 (neox) or 8 (gptj). */
+typedef struct {
+  const float* cos_sin;       /* [device] */
+  const int32_t* rope_idx;    /* [device] */
+  const int32_t* layer_group; /* [device] or null */
+  int32_t n_tables, n_groups, rot_dim, style;
+} dsr_mx_rope;
+
+/* Bytes of one layer of a quantised record; DSR_ERR_ARG or DSR_ERR_SHAPE (< 0). */
+int64_t dsr_mx_layer_bytes(int format, int block_size, int num_heads, int head_dim);
+
+/* Pages -> quantised records and back, layers [first, first + count) of the table
+ * (record layer layer0 + l). As dsr_gather and dsr_scatter / dsr_scatter_rerotate
+ * (rope null: no rotation): a decoded K row is rotated in fp32 and rounded once. */
+int dsr_gather_mx(const dsr_mx_args* args, int first, int count, const int32_t* page_ids,
+                  const int64_t* slot_offsets, int n_pages, dsr_stream_t stream);
+int dsr_scatter_mx(const dsr_mx_args* args, int first, int count, const int32_t* page_ids,
+                   const int64_t* slot_offsets, int n_pages, const dsr_mx_rope* rope,
+                   dsr_stream_t stream);
+
+/* The same by token: cache slot slot_mapping[t] (block * block_size + offset;
+ * negative: skipped) <-> row record_rows[t] = record offset * block_size + row. */
+int dsr_gather_slots_mx(const dsr_mx_args* args, int first, int count,
+                        const int64_t* slot_mapping, const int64_t* record_rows, int n_tokens,
+                        dsr_stream_t stream);
+int dsr_scatter_slots_mx(const dsr_mx_args* args, int first, int count,
+                         const int64_t* slot_mapping, const int64_t* record_rows, int n_tokens,
+                         const dsr_mx_rope* rope, dsr_stream_t stream);
+
+/*
+ * Attention over quantised records, in place of a load into pages:
+ *     out[i, h] = sum_t p_t v_t,  p = softmax_t(scale * q[i, h] . k_t),
+ *     lse[i, h] = log sum_t exp(scale * q[i, h] . k_t)   (natural logarithm)
+ * over the tokens t < min(context[r], limits[i]) of query i's request r, whose
+ * queries are rows q_start[r] .. q_start[r + 1] - 1 and whose tokens lie in order
+ * in the records slot_offsets[page_start[r] .. page_start[r + 1]), block_size to
+ * each. k and v are the records' values as a load into pages of q's type reads
+ * them, k rotated by table rope_idx[page] (-1: not). Query head h reads KV head
+ * h / (q_heads / kv_heads). A query that sees no token gets out 0, lse -inf.
+ *
+ * prior_out / prior_lse (both or neither): the same queries' attention over other
+ * keys, joined with it: out and lse are those over both sets.
+ *
+ * Tokens of a page whose record leaves the staging buffer are not seen; entries of
+ * the start arrays are clamped to their tables, and context to its request's pages.
+ * max_queries and max_context shape the launch: larger requests are computed too,
+ * but run longer. out rows of no request are left as they were.
+ *
+ * q rows of head_dim elements (32, 64, 96, 128 or 256) are contiguous and 16-byte
+ * aligned, their strides in bytes; out and prior_out are contiguous [n_q][q_heads]
+ * [head_dim] of q's type, lse and prior_lse float [n_q][q_heads]. block_size is a
+ * multiple of 16. workspace: dsr_attend_workspace() bytes, 16-byte aligned, free
+ * again when the call's work has run (calls that may overlap need one each).
+ * No counterpart in the reference, whose chunks reach attention through pages only.
+ */
+typedef struct {
+  const void* q;
+  int64_t q_row_stride, q_head_stride;
+  void* out;
+  float* lse;
+  const void* prior_out;
+  const float* prior_lse;
+  const int32_t* q_start;      /* [device] n_req + 1 */
+  const int32_t* page_start;   /* [device] n_req + 1 */
+  const int64_t* slot_offsets; /* [device] n_pages */
+  const int32_t* context;      /* [device] n_req */
+  const int32_t* limits;       /* [device] n_q, or null */
+  const int32_t* rope_idx;     /* [device] n_pages, or null: nothing is rotated */
+  const float* cos_sin;        /* [device] n_tables * (rot_dim / 2) pairs */
+  const void* staging;
+  int64_t staging_bytes, layer_bytes;
+  void* workspace;
+  int64_t workspace_bytes;
+  float scale;
+  int32_t n_req, n_q, n_pages, max_queries, max_context;
+  int32_t q_heads, kv_heads, head_dim, block_size, layer;
+  int32_t n_tables, rot_dim, style;
+  int32_t dtype, format;
+} dsr_attend_args;
+
+int64_t dsr_attend_workspace(const dsr_attend_args* args);
+int dsr_attend_mx(const dsr_attend_args* args, dsr_stream_t stream);
 
 /*
  * Pinned-host staging ring between device records and the store file.
