@@ -5,8 +5,18 @@
 // in place. A moved chunk's keys R(d) k meet the queries as q . R(d) k = (R(-d) q) . k,
 // so the query is rotated, once per chunk, and the keys are not.
 //
-// One wave per (query row, head): 64 tokens at a time, each lane one token's score,
-// then each lane D / 64 columns of the values.
+// A workgroup takes one request, one KV head, a tile of 16 NQ query rows (query tokens
+// times the heads that share the KV head) and a stretch of the tokens; its 4 waves take
+// turns at steps of 32 tokens. Per step and wave:
+//   S^T = K Q^T    tokens x rows, so that a lane holds 4 consecutive tokens of one row.
+//                  Lane (n, g) dequantises the quarter g of row n, one 16-byte load of
+//                  e2m1 at head_dim 128, and the MFMA's k index runs over the quarters.
+//   P              exponentials against a running maximum that is renewed only when a
+//                  score passes it by 2^8, so that the usual step has no reduction.
+//   O^T += V^T P^T P^T is in the MFMA's operand layout as it comes from S^T. V is
+//                  dequantised to LDS row by row and read back transposed
+//                  (ds_read_b64_tr_b16); the wave uses its own part, without barriers.
+// K and V are exact in q's type, products and sums are fp32, P is rounded to q's type.
 
 #pragma once
 
@@ -18,139 +28,589 @@ struct AttendArgs {
   dsr_attend_args a;
   int32_t codes, scales;  // section bytes of one half
   int64_t need;
+  int32_t group;          // query heads per KV head
+  int32_t tiles, splits;  // of blockIdx.x
+  int32_t chunk;          // tokens of a split (the last one takes the rest)
+  float scale2;           // scale * log2(e)
+  float* part_o;          // [n_q * q_heads][splits][head_dim]
+  float2* part_ml;        // [n_q * q_heads][splits] (maximum in log2 units, sum)
 };
-
-template <int FMT>
-__device__ __forceinline__ float mx_element(const uint8_t* codes, const uint8_t* scales,
-                                            int64_t i) {
-  const uint32_t s = scales[i >> 5];
-  if (s == 255u) return __uint_as_float(0x7fc00000u);
-  if (FMT == DSR_MX_INT8) return __builtin_ldexpf((float)(int8_t)codes[i], (int)s - 133);
-  const uint32_t c = codes[i >> 1] >> (4 * (i & 1)) & 15u;
-  const uint32_t e = c >> 1 & 3u, f = c & 1u;
-  const float m = e ? __builtin_ldexpf(1.0f + 0.5f * f, (int)e - 1) : 0.5f * f;
-  return __builtin_ldexpf(c & 8u ? -m : m, (int)s - 127);
-}
 
 template <int DT>
 __device__ __forceinline__ float read16(const void* p, int64_t i) {
   const uint32_t h = static_cast<const uint16_t*>(p)[i];
   return DT == DSR_DTYPE_BF16 ? bf16_to_f32(h) : fp16_to_f32(h);
 }
-template <int DT>
-__device__ __forceinline__ float as_type(float f) {  // as a cache of the type holds it
-  const float top = DT == DSR_DTYPE_BF16 ? __uint_as_float(0x7f7f0000u) : 65504.0f;
-  f = f > top ? top : f;
-  f = f < -top ? -top : f;
-  return DT == DSR_DTYPE_BF16 ? bf16_to_f32(f32_to_bf16(f)) : fp16_to_f32(f32_to_fp16(f));
-}
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) {
   return x < lo ? lo : x > hi ? hi : x;
 }
 
+// Request r: its query rows [q0, q1), its pages from p0, its tokens.
+struct AttendRequest {
+  int q0, q1, p0;
+  int64_t tokens;
+};
+__device__ __forceinline__ AttendRequest attend_request(const dsr_attend_args& a, int r) {
+  AttendRequest o;
+  o.q0 = clampi(a.q_start[r], 0, a.n_q);
+  o.q1 = clampi(a.q_start[r + 1], 0, a.n_q);
+  o.p0 = clampi(a.page_start[r], 0, a.n_pages);
+  const int p1 = clampi(a.page_start[r + 1], o.p0, a.n_pages);
+  const int64_t held = (int64_t)(p1 - o.p0) * a.block_size;
+  o.tokens = a.context[r];
+  o.tokens = o.tokens < 0 ? 0 : o.tokens > held ? held : o.tokens;
+  return o;
+}
+
+// 2^x; log2.
+__device__ __forceinline__ float exp2_(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float log2_(float x) { return __builtin_amdgcn_logf(x); }
+constexpr float kLn2 = 0.69314718055994531f;
+
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+
+template <int DT>
+__device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
+  if constexpr (DT == DSR_DTYPE_BF16)
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// Two floats as q's type, round to nearest even.
+template <int DT>
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  const f32x2 f = {x, y};
+  if constexpr (DT == DSR_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
+}
+template <int DT>
+__device__ __forceinline__ float half_of(uint32_t w, int k) {
+  const uint32_t h = k ? w >> 16 : w & 0xffffu;
+  return DT == DSR_DTYPE_BF16 ? bf16_to_f32(h) : fp16_to_f32(h);
+}
+
+// Scale codes above it may read as more than q's type holds (and 255 as NaN): such blocks
+// take the path that saturates.
 template <int FMT, int DT>
-__global__ __launch_bounds__(kWave) void kv_mx_attend_simple_kernel(AttendArgs g) {
-  const dsr_attend_args& a = g.a;
-  const int lane = (int)threadIdx.x, hq = (int)blockIdx.y, r = (int)blockIdx.z;
-  const int D = a.head_dim, bs = a.block_size;
-  const int h = hq / (a.q_heads / a.kv_heads);
-  __shared__ float qs[256], ps[kWave];
-  const int q0 = clampi(a.q_start[r], 0, a.n_q), q1 = clampi(a.q_start[r + 1], 0, a.n_q);
-  const int p0 = clampi(a.page_start[r], 0, a.n_pages);
-  const int p1 = clampi(a.page_start[r + 1], p0, a.n_pages);
+__device__ __forceinline__ constexpr uint32_t top_scale() {
+  return DT == DSR_DTYPE_BF16 ? (FMT == DSR_MX_FP4 ? 252u : 254u)
+                              : (FMT == DSR_MX_FP4 ? 140u : 142u);
+}
+
+// 8 codes (w[0], and w[1] of int8) under scale code s as 8 values of q's type.
+template <int FMT, int DT>
+__device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
+  u32x4 o;
+  if constexpr (FMT == DSR_MX_FP4) {
+    const float scale = mx_scale(s);
+#define DSR_DQ(K)                                                                            \
+  if constexpr (DT == DSR_DTYPE_BF16)                                                        \
+    o[K] = __builtin_bit_cast(uint32_t,                                                      \
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, K));    \
+  else                                                                                       \
+    o[K] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], scale, K));
+    DSR_DQ(0)
+    DSR_DQ(1)
+    DSR_DQ(2)
+    DSR_DQ(3)
+#undef DSR_DQ
+  } else {
+    const int e = (int)s - 133;
+    // small scales are subnormal themselves: the power is applied in two steps
+    const float lo = __builtin_ldexpf(1.0f, e < -100 ? e + 64 : e);
+    const float hi = e < -100 ? 0x1p-64f : 1.0f;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint32_t x = w[k >> 1] >> (16 * (k & 1));
+      o[k] = pack2<DT>((float)(int8_t)x * lo * hi, (float)(int8_t)(x >> 8) * lo * hi);
+    }
+  }
+  return o;
+}
+template <int FMT, int DT>
+__device__ __forceinline__ u32x4 dequantise_saturated(const uint32_t* w, uint32_t s) {
+  float x[8];
+  mx_decode<FMT>(uint2{w[0], FMT == DSR_MX_FP4 ? 0u : w[1]}, s, x);
+  return mx_store_vec<DT>(x);
+}
+
+// out[i][h] and its lse from the unnormalised sum o (4 consecutive columns from d on),
+// the maximum m (log2 units) and the sum l of this kernel's part, and the prior's.
+struct AttendScale {
+  float own, other, lse;
+};
+__device__ __forceinline__ AttendScale attend_scale(const dsr_attend_args& a, int64_t at, float m,
+                                                    float l) {
   const float ninf = -__builtin_inff();
-  for (int i = q0 + (int)blockIdx.x; i < q1; i += (int)gridDim.x) {
-    int64_t ctx = a.context[r];
-    if (a.limits && a.limits[i] < ctx) ctx = a.limits[i];
-    if (ctx > (int64_t)(p1 - p0) * bs) ctx = (int64_t)(p1 - p0) * bs;
-    const uint8_t* q = static_cast<const uint8_t*>(a.q) + (int64_t)i * a.q_row_stride +
-                       (int64_t)hq * a.q_head_stride;
-    float m = ninf, sum = 0.0f, acc[4] = {0, 0, 0, 0};
-    int table = -2;
-    for (int64_t t0 = 0; t0 < ctx; t0 += bs) {  // a page at a time
-      const int p = p0 + (int)(t0 / bs);
-      const int64_t at = a.slot_offsets[p], off = at + (int64_t)a.layer * a.layer_bytes;
-      if (at < 0 || (off & 15) || off + g.need > a.staging_bytes) continue;
-      const uint8_t* rec = static_cast<const uint8_t*>(a.staging) + off;
-      int ti = a.rope_idx ? a.rope_idx[p] : -1;
-      if (ti >= a.n_tables) ti = -1;
-      if (ti != table) {
-        __syncthreads();
-        const float2* cs = reinterpret_cast<const float2*>(a.cos_sin) + (int64_t)ti * (a.rot_dim / 2);
-        for (int d = lane; d < D; d += kWave) {
-          float x = read16<DT>(q, d);
-          if (ti >= 0 && d < a.rot_dim) {
-            const int half = a.rot_dim / 2;
-            const bool neox = a.style == DSR_ROPE_NEOX;
-            const bool lower = neox ? d < half : (d & 1) == 0;
-            const float y = read16<DT>(q, neox ? (lower ? d + half : d - half) : d ^ 1);
-            const float2 w = cs[neox ? (lower ? d : d - half) : d >> 1];
-            x = x * w.x + (lower ? y * w.y : -(y * w.y));  // by -delta
+  AttendScale o;
+  o.lse = l == 0.0f ? ninf : (m + log2_(l)) * kLn2;
+  o.own = l == 0.0f ? 0.0f : 1.0f / l;
+  o.other = 0.0f;
+  if (a.prior_out) {
+    const float l2 = a.prior_lse[at];
+    const float top = l2 > o.lse ? l2 : o.lse;
+    if (top != ninf) {
+      const float e1 = exp2_((o.lse - top) / kLn2), e2 = exp2_((l2 - top) / kLn2);
+      o.own *= e1 / (e1 + e2);
+      o.other = e2 / (e1 + e2);
+      o.lse = top + log2_(e1 + e2) * kLn2;
+    }
+  }
+  return o;
+}
+template <int DT>
+__device__ __forceinline__ void attend_store(const dsr_attend_args& a, int64_t at, int d, f32x4 o,
+                                             const AttendScale& s) {
+  const int64_t i = at * a.head_dim + d;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    o[k] = s.own == 0.0f ? 0.0f : o[k] * s.own;
+    if (s.other != 0.0f) o[k] += s.other * read16<DT>(a.prior_out, i + k);
+  }
+  uint2 w{pack2<DT>(o[0], o[1]), pack2<DT>(o[2], o[3])};
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + i) = w;
+}
+
+// One 16-token tile as loaded: this lane's quarter of K row and V row n, and their scales.
+template <int FMT, int D>
+struct AttendTile {
+  static constexpr int W = (FMT == DSR_MX_FP4 ? 1 : 2) * (D / 32);  // dwords of a quarter
+  static constexpr int S = D == 96 || D == 256 ? 2 : 1;             // blocks it touches
+  uint32_t k[W], v[W];
+  uint32_t ks[S], vs[S];
+};
+
+template <int W>
+__device__ __forceinline__ void load_words(rsrc_t r, int off, uint32_t* w) {
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  typedef unsigned int u32x3 __attribute__((ext_vector_type(3)));
+  int i = 0;
+  if constexpr (W >= 4) {
+#pragma unroll
+    for (int k = 0; k < W / 4; ++k, i += 4) {
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, 0, 0);
+      w[i] = x[0];
+      w[i + 1] = x[1];
+      w[i + 2] = x[2];
+      w[i + 3] = x[3];
+    }
+  }
+  constexpr int rest = W % 4, at = W / 4 * 4;
+  if constexpr (rest == 1) w[at] = __builtin_amdgcn_raw_buffer_load_b32(r, off + 4 * at, 0, 0);
+  if constexpr (rest == 2) {
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off + 4 * at, 0, 0);
+    w[at] = x[0];
+    w[at + 1] = x[1];
+  }
+  if constexpr (rest == 3) {
+    const u32x3 x = __builtin_amdgcn_raw_buffer_load_b96(r, off + 4 * at, 0, 0);
+    w[at] = x[0];
+    w[at + 1] = x[1];
+    w[at + 2] = x[2];
+  }
+}
+
+// Query rows of this lane's column as MFMA operands: chunk i of quarter g, rotated by
+// -delta with table cs (null: as they are); lo: what the rounding of hi left.
+template <int DT, int D, bool ROPE>
+__device__ __forceinline__ void load_query(const dsr_attend_args& a, const uint8_t* row, int quarter,
+                                           const float2* cs, u32x4* hi, u32x4* lo) {
+  constexpr int B = D / 32;
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    const int c = quarter * B + i;  // 8 elements
+    u32x4 x = row ? *reinterpret_cast<const u32x4*>(row + 16 * c) : u32x4{0u, 0u, 0u, 0u};
+    if constexpr (ROPE) lo[i] = u32x4{0u, 0u, 0u, 0u};
+    if (ROPE && cs && row && c * 8 < a.rot_dim) {
+      const bool neox = a.style == DSR_ROPE_NEOX;
+      const int half = a.rot_dim / 16;  // chunks to the neox partner
+      const bool lower = c < half;
+      const u32x4 y = neox ? *reinterpret_cast<const u32x4*>(row + 16 * (lower ? c + half : c - half))
+                           : x;
+      const float2* t = cs + (neox ? (lower ? c : c - half) * 8 : c * 4);
+      u32x4 h, l;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float x0 = half_of<DT>(x[k], 0), x1 = half_of<DT>(x[k], 1);
+        float r0, r1;
+        if (neox) {
+          const float2 t0 = t[2 * k], t1 = t[2 * k + 1];
+          const float y0 = half_of<DT>(y[k], 0), y1 = half_of<DT>(y[k], 1);
+          r0 = lower ? x0 * t0.x + y0 * t0.y : x0 * t0.x - y0 * t0.y;
+          r1 = lower ? x1 * t1.x + y1 * t1.y : x1 * t1.x - y1 * t1.y;
+        } else {
+          const float2 t0 = t[k];
+          r0 = x0 * t0.x + x1 * t0.y;
+          r1 = x1 * t0.x - x0 * t0.y;
+        }
+        h[k] = pack2<DT>(r0, r1);
+        l[k] = pack2<DT>(r0 - half_of<DT>(h[k], 0), r1 - half_of<DT>(h[k], 1));
+      }
+      x = h;
+      lo[i] = l;
+    }
+    hi[i] = x;
+  }
+}
+
+constexpr int kAttendWaves = 4;
+constexpr int kStep = 32;  // tokens of a step
+
+// 16-byte chunks of a V row in LDS, and the place of chunk c of row n. Writes put one
+// chunk of 16 rows down together, transposing reads take two neighbouring chunks of 8
+// rows: under this permutation both meet each bank once.
+template <int D>
+__device__ __forceinline__ constexpr int lds_chunks() {
+  return D <= 64 ? 8 : D <= 128 ? 16 : 32;
+}
+template <int D>
+__device__ __forceinline__ int lds_place(int n, int c) {
+  if constexpr (D <= 64) return n * 8 + (c ^ (((n >> 1) & 3) << 1 | ((n >> 3) & 1)));
+  return n * lds_chunks<D>() + (c ^ ((n & 7) << 1 | ((n >> 3) & 1)));
+}
+
+template <int FMT, int DT, int D, int NQ, bool ROPE>
+__global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
+  const dsr_attend_args& a = g.a;
+  constexpr int B = D / 32, NT = D / 16;
+  using Tile = AttendTile<FMT, D>;
+  __shared__ u32x4 lds[kAttendWaves * kStep * lds_chunks<D>()];
+  __shared__ float2 lds_ml[kAttendWaves][16];
+  const int lane = (int)threadIdx.x % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+  const int n = lane & 15, quarter = lane >> 4;
+  u32x4* const mine = lds + wave * kStep * lds_chunks<D>();
+  const int h = (int)blockIdx.y;
+  const int split = (int)blockIdx.x % g.splits, tile0 = (int)blockIdx.x / g.splits;
+  const AttendRequest rq = attend_request(a, (int)blockIdx.z);
+  const int64_t rows = rq.q1 > rq.q0 ? (int64_t)(rq.q1 - rq.q0) * g.group : 0;
+  const float ninf = -__builtin_inff();
+
+  for (int64_t row0 = (int64_t)tile0 * (16 * NQ); row0 < rows; row0 += (int64_t)g.tiles * (16 * NQ)) {
+    // this lane's columns
+    int lim[NQ];
+    const uint8_t* qrow[NQ];
+    int tmax = 0, tmin = 0x7fffffff;
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      const int64_t row = row0 + 16 * j + n;
+      const bool in = row < rows;
+      const int i = rq.q0 + (int)(row / g.group);
+      lim[j] = 0;
+      qrow[j] = nullptr;
+      if (in) {
+        int64_t seen = rq.tokens;
+        if (a.limits && a.limits[i] < seen) seen = a.limits[i];
+        lim[j] = seen < 0 ? 0 : (int)seen;
+        qrow[j] = static_cast<const uint8_t*>(a.q) + (int64_t)i * a.q_row_stride +
+                  (int64_t)(h * g.group + (int)(row % g.group)) * a.q_head_stride;
+        tmin = lim[j] < tmin ? lim[j] : tmin;
+      }
+      tmax = lim[j] > tmax ? lim[j] : tmax;
+    }
+#pragma unroll
+    for (int k = 1; k < 16; k <<= 1) {
+      const int x = __shfl_xor(tmax, k), y = __shfl_xor(tmin, k);
+      tmax = x > tmax ? x : tmax;
+      tmin = y < tmin ? y : tmin;
+    }
+    tmax = __builtin_amdgcn_readfirstlane(tmax);
+    tmin = __builtin_amdgcn_readfirstlane(tmin);
+    const int64_t begin = (int64_t)split * g.chunk;
+    int64_t end = split == g.splits - 1 ? tmax : begin + g.chunk;
+    if (end > tmax) end = tmax;
+    if (begin >= end && split > 0) continue;  // the join does not read it
+
+    u32x4 qh[NQ][B], ql[ROPE ? NQ : 1][ROPE ? B : 1];
+    int table = -1;
+#pragma unroll
+    for (int j = 0; j < NQ; ++j)
+      load_query<DT, D, ROPE>(a, qrow[j], quarter, nullptr, qh[j], ql[ROPE ? j : 0]);
+    f32x4 acc[NQ][NT];
+    float m[NQ], l[NQ];
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      m[j] = ninf;
+      l[j] = 0.0f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t) acc[j][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+
+    // tile loads: a tile whose record is out of bounds reads zeros and is not seen
+    auto load_tile = [&](int64_t t, Tile* o, bool* seen, int* ti) {
+      const int p = rq.p0 + (int)(t / a.block_size);
+      const bool live = t < end;
+      const int64_t at = live ? a.slot_offsets[p] : -1;
+      const int64_t off = at + (int64_t)a.layer * a.layer_bytes;
+      *seen = live && at >= 0 && (at & 15) == 0 && off + g.need <= a.staging_bytes;
+      *ti = -1;
+      if (ROPE && *seen) {
+        *ti = a.rope_idx[p];
+        if (*ti < -1 || *ti >= a.n_tables) *ti = -1;
+      }
+      const rsrc_t r = make_rsrc(static_cast<const uint8_t*>(a.staging) + (*seen ? off : 0),
+                                 *seen ? g.need : 0);
+      const int row = h * a.block_size + (int)(t % a.block_size) + n;
+      const int at_k = row * (Tile::W * 16) + quarter * (Tile::W * 4);
+      load_words<Tile::W>(r, at_k, o->k);
+      load_words<Tile::W>(r, at_k + g.codes, o->v);
+      const int at_s = 2 * g.codes + row * B;
+      const int b0 = B * quarter / 4, b1 = (B * quarter + B - 1) / 4;
+      o->ks[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b0, 0, 0);
+      o->vs[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b0, 0, 0);
+      if constexpr (Tile::S == 2) {
+        o->ks[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b1, 0, 0);
+        o->vs[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b1, 0, 0);
+      }
+    };
+    // the scale of chunk i of this lane's quarter
+    auto scale_of = [&](const uint32_t* s, int i) -> uint32_t {
+      if constexpr (Tile::S == 1) return s[0];
+      return (B * quarter + i) / 4 == B * quarter / 4 ? s[0] : s[1];
+    };
+    auto odd = [&](const uint32_t* s) -> bool {
+      bool o = s[0] > top_scale<FMT, DT>();
+      if constexpr (Tile::S == 2) o |= s[1] > top_scale<FMT, DT>();
+      return __any(o);
+    };
+
+    for (int64_t t = begin + wave * kStep; t < end; t += kAttendWaves * kStep) {
+      Tile tile[2];
+      bool seen[2];
+      int ti[2];
+      load_tile(t, &tile[0], &seen[0], &ti[0]);
+      load_tile(t + 16, &tile[1], &seen[1], &ti[1]);
+      f32x4 s[NQ][2];
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        if (ROPE && seen[u] && ti[u] != table) {
+          table = ti[u];
+          const float2* cs = table < 0 ? nullptr : reinterpret_cast<const float2*>(a.cos_sin) +
+                                                       (int64_t)table * (a.rot_dim / 2);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+            load_query<DT, D, ROPE>(a, qrow[j], quarter, cs, qh[j], ql[j]);
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        const bool slow = odd(tile[u].ks);
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const uint32_t* w = tile[u].k + i * (Tile::W / B);
+          const uint32_t sc = scale_of(tile[u].ks, i);
+          u32x4 kf;
+          if (__builtin_expect(slow, 0)) kf = dequantise_saturated<FMT, DT>(w, sc);
+          else kf = dequantise<FMT, DT>(w, sc);
+#pragma unroll
+          for (int j = 0; j < NQ; ++j) {
+            s[j][u] = mfma32<DT>(kf, qh[j][i], s[j][u]);
+            if (ROPE && table >= 0) s[j][u] = mfma32<DT>(kf, ql[j][i], s[j][u]);
           }
-          qs[d] = x;
         }
-        table = ti;
-        __syncthreads();
       }
-      const uint8_t* vc = rec + g.codes;
-      const uint8_t* ks = rec + 2 * (int64_t)g.codes;
-      const uint8_t* vs = ks + g.scales;
-      for (int b = 0; b < bs && t0 + b < ctx; b += kWave) {
-        const int n = bs - b < kWave ? bs - b : kWave;
-        const bool seen = lane < n && t0 + b + lane < ctx;
-        float s = ninf;
-        if (seen) {
-          s = 0.0f;
-          const int64_t row = ((int64_t)h * bs + b + lane) * D;
-          for (int d = 0; d < D; ++d) s += qs[d] * as_type<DT>(mx_element<FMT>(rec, ks, row + d));
-          s *= a.scale;
+
+      // V of both tiles to LDS, its NaN blocks as zeros that are put back below
+      bool any_nan = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const bool slow = odd(tile[u].vs);
+        const int64_t tok = t + 16 * u + n;
+        const bool row_in = seen[u] && tok < tmax;
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
+          const uint32_t* w = tile[u].v + i * (Tile::W / B);
+          const uint32_t sc = scale_of(tile[u].vs, i);
+          u32x4 vf;
+          if (__builtin_expect(slow, 0)) {
+            vf = dequantise_saturated<FMT, DT>(w, sc);
+            if (sc == 255u || !row_in) vf = u32x4{0u, 0u, 0u, 0u};
+          } else {
+            vf = dequantise<FMT, DT>(w, sc);
+          }
+          mine[lds_place<D>(16 * u + n, quarter * B + i)] = vf;
         }
-        float top = s;
-        for (int k = 32; k; k >>= 1) {
-          const float o = __shfl_xor(top, k);
-          top = top > o || __builtin_isnan(top) ? top : o;  // a NaN stays
+        any_nan |= slow;
+      }
+
+      // P
+      const bool masked = t + kStep > tmin || !seen[0] || !seen[1];
+      u32x4 pf[NQ];
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        float x[8];
+        const float base = m[j] == ninf ? 0.0f : m[j];
+        float top = ninf;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_fmaf(s[j][e >> 2][e & 3], g.scale2, -base);
+          if (masked) {
+            const int64_t tok = t + 16 * (e >> 2) + 4 * quarter + (e & 3);
+            if (tok >= lim[j] || !seen[e >> 2]) x[e] = ninf;
+          }
+          top = __builtin_fmaxf(top, x[e]);
         }
-        const float mn = m > top || __builtin_isnan(m) ? m : top;
-        const float keep = m == ninf ? 0.0f : __expf(m - mn);
-        const float pr = seen ? __expf(s - mn) : 0.0f;
-        float part = pr;
-        for (int k = 32; k; k >>= 1) part += __shfl_xor(part, k);
-        sum = sum * keep + part;
-        m = mn;
-        __syncthreads();
-        ps[lane] = pr;
-        __syncthreads();
-        for (int j = 0; j * kWave < D; ++j) {
-          const int d = j * kWave + lane;
-          acc[j] *= keep;
-          if (d >= D) continue;
-          for (int t = 0; t < n && t0 + b + t < ctx; ++t)
-            acc[j] += ps[t] * as_type<DT>(mx_element<FMT>(vc, vs, ((int64_t)h * bs + b + t) * D + d));
+        if (__any(top > 8.0f || (m[j] == ninf && top > ninf))) {
+          float o = __shfl_xor(top, 16);
+          top = __builtin_fmaxf(top, o);
+          o = __shfl_xor(top, 32);
+          top = __builtin_fmaxf(top, o);
+          const float mn = __builtin_fmaxf(m[j], top + base);
+          if (mn != ninf) {
+            const float keep = exp2_(m[j] - mn);
+            const float shift = mn - base;
+            m[j] = mn;
+            l[j] *= keep;
+#pragma unroll
+            for (int k = 0; k < NT; ++k) acc[j][k] *= keep;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] -= shift;
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          x[e] = exp2_(x[e]);
+          l[j] += x[e];
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) pf[j][k] = pack2<DT>(x[2 * k], x[2 * k + 1]);
+      }
+
+      // O^T: lanes' columns 4 c ... of rows 4 quarter + r, transposed in 16-lane groups
+#pragma unroll
+      for (int k = 0; k < NT; ++k) {
+        union {
+          s16x4 h[2];
+          u32x4 v;
+        } vt;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int row = 16 * u + 4 * quarter + (n >> 2);
+          const int place = lds_place<D>(row, 2 * k + ((n & 3) >> 1)) * 16 + (n & 1) * 8;
+          vt.h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(reinterpret_cast<char*>(mine) + place));
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) acc[j][k] = mfma32<DT>(vt.v, pf[j], acc[j][k]);
+      }
+
+      if (__builtin_expect(any_nan, 0)) {
+        const float nan = __uint_as_float(0x7fc00000u);
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+          for (int b = 0; b < B; ++b) {
+            // lanes whose quarter begins in block b, or reaches it
+            bool bad = tile[u].vs[0] == 255u && B * quarter / 4 == b;
+            if constexpr (Tile::S == 2)
+              bad |= tile[u].vs[1] == 255u && (B * quarter + B - 1) / 4 == b;
+            uint64_t rows_nan = __ballot(bad && seen[u]);
+            rows_nan |= rows_nan >> 32;
+            rows_nan |= rows_nan >> 16;
+            uint32_t left = (uint32_t)rows_nan & 0xffffu;
+            while (left) {
+              const int64_t tok = t + 16 * u + __builtin_ctz(left);
+              left &= left - 1;
+#pragma unroll
+              for (int j = 0; j < NQ; ++j)
+                if (tok < lim[j]) {
+                  acc[j][2 * b] = f32x4{nan, nan, nan, nan};
+                  acc[j][2 * b + 1] = f32x4{nan, nan, nan, nan};
+                }
+            }
+          }
         }
       }
     }
-    float lse = m == ninf ? ninf : m + __logf(sum);
-    float own = sum > 0.0f || __builtin_isnan(sum) ? 1.0f / sum : 0.0f, other = 0.0f;
+
+    // the 4 waves joined, 16 rows at a time
+#pragma unroll
+    for (int j = 0; j < NQ; ++j) {
+      l[j] += __shfl_xor(l[j], 16);
+      l[j] += __shfl_xor(l[j], 32);
+      __syncthreads();
+      if (quarter == 0) lds_ml[wave][n] = float2{m[j], l[j]};
+      float* o = reinterpret_cast<float*>(lds) + wave * (D * 16);
+#pragma unroll
+      for (int k = 0; k < NT; ++k)
+        *reinterpret_cast<f32x4*>(o + n * D + ((16 * k + 4 * quarter) ^ ((n & 7) << 2))) = acc[j][k];
+      __syncthreads();
+      const int col = (int)threadIdx.x >> 4;
+      const int64_t row = row0 + 16 * j + col;
+      if (row < rows) {
+        float mt = ninf, lt = 0.0f, f[kAttendWaves];
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; ++w) mt = __builtin_fmaxf(mt, lds_ml[w][col].x);
+#pragma unroll
+        for (int w = 0; w < kAttendWaves; ++w) {
+          const float2 ml = lds_ml[w][col];
+          f[w] = ml.y == 0.0f ? 0.0f : exp2_(ml.x - mt);
+          lt += ml.y * f[w];
+        }
+        const int i = rq.q0 + (int)(row / g.group);
+        const int64_t at = (int64_t)i * a.q_heads + h * g.group + (int)(row % g.group);
+        AttendScale sc{};
+        if (g.splits == 1) {
+          sc = attend_scale(a, at, mt, lt);
+          if ((threadIdx.x & 15) == 0) a.lse[at] = sc.lse;
+        } else if ((threadIdx.x & 15) == 0) {
+          g.part_ml[at * g.splits + split] = float2{mt, lt};
+        }
+        for (int d = ((int)threadIdx.x & 15) * 4; d < D; d += 64) {
+          f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int w = 0; w < kAttendWaves; ++w) {
+            const f32x4 x = *reinterpret_cast<const f32x4*>(
+                reinterpret_cast<const float*>(lds) + w * (D * 16) + col * D + (d ^ ((col & 7) << 2)));
+            sum += x * f[w];
+          }
+          if (g.splits == 1) attend_store<DT>(a, at, d, sum, sc);
+          else *reinterpret_cast<f32x4*>(g.part_o + (at * g.splits + split) * D + d) = sum;
+        }
+      }
+    }
+    __syncthreads();
+  }
+}
+
+// The splits of a row joined in their order: 16 lanes to a row.
+template <int DT>
+__global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs g) {
+  const dsr_attend_args& a = g.a;
+  const AttendRequest rq = attend_request(a, (int)blockIdx.z);
+  const int sub = (int)threadIdx.x & 15;
+  const int hq = (int)blockIdx.y * (kThreads / 16) + ((int)threadIdx.x >> 4);
+  if (hq >= a.q_heads) return;
+  const float ninf = -__builtin_inff();
+  for (int i = rq.q0 + (int)blockIdx.x; i < rq.q1; i += (int)gridDim.x) {
     const int64_t at = (int64_t)i * a.q_heads + hq;
-    if (a.prior_out) {
-      const float l2 = a.prior_lse[at], top = l2 > lse ? l2 : lse;
-      if (top != ninf) {
-        const float e1 = __expf(lse - top), e2 = __expf(l2 - top);
-        own *= e1 / (e1 + e2);
-        other = e2 / (e1 + e2);
-        lse = top + __logf(e1 + e2);
+    int64_t seen = rq.tokens;
+    if (a.limits && a.limits[i] < seen) seen = a.limits[i];
+    int64_t n = seen <= 0 ? 0 : (seen + g.chunk - 1) / g.chunk;
+    if (n > g.splits) n = g.splits;
+    float m = ninf, l = 0.0f;
+    const float2* ml = g.part_ml + at * g.splits;
+    for (int s = 0; s < n; ++s) m = __builtin_fmaxf(m, ml[s].x);
+    for (int s = 0; s < n; ++s) l += ml[s].y == 0.0f ? 0.0f : ml[s].y * exp2_(ml[s].x - m);
+    const AttendScale sc = attend_scale(a, at, m, l);
+    if (sub == 0) a.lse[at] = sc.lse;
+    for (int d = sub * 4; d < a.head_dim; d += 64) {
+      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+      for (int s = 0; s < n; ++s) {
+        if (ml[s].y == 0.0f) continue;
+        sum += *reinterpret_cast<const f32x4*>(g.part_o + (at * g.splits + s) * a.head_dim + d) *
+               exp2_(ml[s].x - m);
       }
+      attend_store<DT>(a, at, d, sum, sc);
     }
-    for (int j = 0; j * kWave < D; ++j) {
-      const int d = j * kWave + lane;
-      if (d >= D) continue;
-      float o = acc[j] * own;
-      if (other != 0.0f) o += other * read16<DT>(a.prior_out, at * D + d);
-      static_cast<uint16_t*>(a.out)[at * D + d] =
-          (uint16_t)(DT == DSR_DTYPE_BF16 ? f32_to_bf16(o) : f32_to_fp16(o));
-    }
-    if (lane == 0) a.lse[at] = lse;
   }
 }
 
