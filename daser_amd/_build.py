@@ -11,11 +11,13 @@ import os
 import shutil
 import subprocess
 import sys
+import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 SRCS = [os.path.join(HERE, "csrc", n)
-        for n in ("kv_move.hip", "kv_mx.hip", "store_ring.cpp", "load_plan.cpp")]
+        for n in ("kv_move.hip", "kv_mx.hip", "kv_attend.hip", "store_ring.cpp", "load_plan.cpp")]
 INCLUDE = os.path.join(ROOT, "include")
 OUT = os.path.join(HERE, "libdaser_kv.so")
 ABI_TEST_SRC = os.path.join(ROOT, "tests", "c", "abi_roundtrip.cpp")
@@ -49,15 +51,23 @@ def hipcc() -> str:
     raise RuntimeError("hipcc not found; the HIP library cannot be built")
 
 
-def build(verbose: bool = False) -> str:
-    """Compiles the kernels and C ABI into ``daser_amd/libdaser_kv.so``."""
-    tmp = OUT + ".tmp"
-    cmd = [hipcc(), *HIPCC_FLAGS, f"-I{INCLUDE}", *SRCS, "-o", tmp]
+def _run(cmd: list[str], verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     proc = subprocess.run(cmd, capture_output=True, text=True)
     if proc.returncode != 0:
         raise RuntimeError(f"hipcc failed ({proc.returncode}):\n{proc.stderr}")
+
+
+def build(verbose: bool = False) -> str:
+    """Compiles the kernels and C ABI into ``daser_amd/libdaser_kv.so``."""
+    tmp = OUT + ".tmp"
+    with tempfile.TemporaryDirectory() as objs, ThreadPoolExecutor(len(SRCS)) as pool:
+        flags = [f for f in HIPCC_FLAGS if f != "-shared"]
+        outs = [os.path.join(objs, os.path.basename(src) + ".o") for src in SRCS]
+        list(pool.map(lambda s, o: _run([hipcc(), *flags, f"-I{INCLUDE}", "-c", s, "-o", o],
+                                        verbose), SRCS, outs))
+        _run([hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", *outs, "-o", tmp], verbose)
     os.replace(tmp, OUT)
     # a C++ caller of the C ABI (no Python, no torch), run by the GPU tests
     cmd = [hipcc(), "-O2", "-std=c++17", f"-I{INCLUDE}", ABI_TEST_SRC, "-o", ABI_TEST_OUT + ".tmp",
@@ -89,7 +99,7 @@ def build_ring_sanitize(verbose: bool = False) -> None:
         return
     cmd = [clang, "-O1", "-g", "-fsanitize=address,undefined", "-fno-omit-frame-pointer",
            "-std=c++17", "-D__HIP_PLATFORM_AMD__", "-I/opt/rocm/include", f"-I{INCLUDE}",
-           SRCS[2], RING_SAN_SRC, "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib",
+           SRCS[3], RING_SAN_SRC, "-L/opt/rocm/lib", "-lamdhip64", "-Wl,-rpath,/opt/rocm/lib",
            "-o", RING_SAN_OUT + ".tmp"]
     if verbose:
         print(" ".join(cmd), flush=True)

@@ -1,5 +1,5 @@
 // kv_attend.h -- attention over quantised records.
-// Part of libdaser_kv: included by kv_mx.hip.
+// Part of libdaser_kv: included by kv_attend.hip.
 //
 // out = sum_t p_t v_t, p = softmax(scale q . R(d) k_t): the records' rows are read
 // in place. A moved chunk's keys R(d) k meet the queries as q . R(d) k = (R(-d) q) . k,
@@ -32,6 +32,7 @@ struct AttendArgs {
   int32_t tiles, splits;  // of blockIdx.x
   int32_t chunk;          // tokens of a split (the last one takes the rest)
   float scale2;           // scale * log2(e)
+  FastDiv by_block;       // tokens to pages
   float* part_o;          // [n_q * q_heads][splits][head_dim]
   float2* part_ml;        // [n_q * q_heads][splits] (maximum in log2 units, sum)
 };
@@ -46,9 +47,11 @@ __device__ __forceinline__ int clampi(int x, int lo, int hi) {
   return x < lo ? lo : x > hi ? hi : x;
 }
 
+constexpr int kMaxTokens = 0x7fff0000;  // of a request, that 32 more are an int too
+
 // Request r: its query rows [q0, q1), its pages from p0, its tokens.
 struct AttendRequest {
-  int q0, q1, p0;
+  int q0, q1, p0, p1;
   int64_t tokens;
 };
 __device__ __forceinline__ AttendRequest attend_request(const dsr_attend_args& a, int r) {
@@ -56,10 +59,11 @@ __device__ __forceinline__ AttendRequest attend_request(const dsr_attend_args& a
   o.q0 = clampi(a.q_start[r], 0, a.n_q);
   o.q1 = clampi(a.q_start[r + 1], 0, a.n_q);
   o.p0 = clampi(a.page_start[r], 0, a.n_pages);
-  const int p1 = clampi(a.page_start[r + 1], o.p0, a.n_pages);
-  const int64_t held = (int64_t)(p1 - o.p0) * a.block_size;
+  o.p1 = clampi(a.page_start[r + 1], o.p0, a.n_pages);
+  const int64_t held = (int64_t)(o.p1 - o.p0) * a.block_size;
   o.tokens = a.context[r];
   o.tokens = o.tokens < 0 ? 0 : o.tokens > held ? held : o.tokens;
+  if (o.tokens > kMaxTokens) o.tokens = kMaxTokens;
   return o;
 }
 
@@ -136,11 +140,19 @@ __device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
   }
   return o;
 }
-template <int FMT, int DT>
-__device__ __forceinline__ u32x4 dequantise_saturated(const uint32_t* w, uint32_t s) {
-  float x[8];
-  mx_decode<FMT>(uint2{w[0], FMT == DSR_MX_FP4 ? 0u : w[1]}, s, x);
-  return mx_store_vec<DT>(x);
+// The same for blocks above top_scale(): saturated; NaN under 255.
+template <int DT>
+__device__ __forceinline__ u32x4 saturate(u32x4 v, uint32_t s) {
+  constexpr uint32_t top = DT == DSR_DTYPE_BF16 ? 0x7f7f7f7fu : 0x7bff7bffu;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t mag = v[k] & 0x7fff7fffu;
+    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, mag),
+                                              __builtin_bit_cast(u16x2, top));
+    v[k] = s == 255u ? (DT == DSR_DTYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u)
+                     : (v[k] & 0x80008000u) | __builtin_bit_cast(uint32_t, m);
+  }
+  return v;
 }
 
 // out[i][h] and its lse from the unnormalised sum o (4 consecutive columns from d on),
@@ -217,6 +229,39 @@ __device__ __forceinline__ void load_words(rsrc_t r, int off, uint32_t* w) {
     w[at + 1] = x[1];
     w[at + 2] = x[2];
   }
+}
+
+// Entries of 64 pages, one to a lane: the offset of the page's layer (-1: not there, or
+// outside the records) and its table.
+struct AttendPages {
+  int64_t off;
+  int table;
+};
+struct AttendPage {
+  int64_t off;
+  int table;
+};
+template <bool ROPE>
+__device__ __forceinline__ AttendPages attend_pages(const AttendArgs& g, const AttendRequest& rq,
+                                                    int page, int lane) {
+  const dsr_attend_args& a = g.a;
+  AttendPages o{-1, -1};
+  const int64_t p = (int64_t)rq.p0 + page + lane;
+  if (p < rq.p1) {
+    const int64_t at = a.slot_offsets[p], off = at + (int64_t)a.layer * a.layer_bytes;
+    if (at >= 0 && (at & 15) == 0 && off + g.need <= a.staging_bytes) o.off = off;
+    if (ROPE) {
+      o.table = a.rope_idx[p];
+      if (o.table < -1 || o.table >= a.n_tables) o.table = -1;
+    }
+  }
+  return o;
+}
+template <bool ROPE>
+__device__ __forceinline__ AttendPage page_of(const AttendPages& x, int i) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)x.off, i);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(x.off >> 32), i);
+  return {(int64_t)((uint64_t)hi << 32 | lo), ROPE ? __builtin_amdgcn_readlane(x.table, i) : -1};
 }
 
 // Query rows of this lane's column as MFMA operands: chunk i of quarter g, rotated by
@@ -325,13 +370,13 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
     }
     tmax = __builtin_amdgcn_readfirstlane(tmax);
     tmin = __builtin_amdgcn_readfirstlane(tmin);
-    const int64_t begin = (int64_t)split * g.chunk;
-    int64_t end = split == g.splits - 1 ? tmax : begin + g.chunk;
-    if (end > tmax) end = tmax;
+    const int64_t begin64 = (int64_t)split * g.chunk;
+    const int begin = begin64 < tmax ? (int)begin64 : tmax;
+    int end = tmax;
+    if (split < g.splits - 1 && tmax - begin > g.chunk) end = begin + g.chunk;
     if (begin >= end && split > 0) continue;  // the join does not read it
 
     u32x4 qh[NQ][B], ql[ROPE ? NQ : 1][ROPE ? B : 1];
-    int table = -1;
 #pragma unroll
     for (int j = 0; j < NQ; ++j)
       load_query<DT, D, ROPE>(a, qrow[j], quarter, nullptr, qh[j], ql[ROPE ? j : 0]);
@@ -345,31 +390,51 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
       for (int t = 0; t < NT; ++t) acc[j][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // tile loads: a tile whose record is out of bounds reads zeros and is not seen
-    auto load_tile = [&](int64_t t, Tile* o, bool* seen, int* ti) {
-      const int p = rq.p0 + (int)(t / a.block_size);
-      const bool live = t < end;
-      const int64_t at = live ? a.slot_offsets[p] : -1;
-      const int64_t off = at + (int64_t)a.layer * a.layer_bytes;
-      *seen = live && at >= 0 && (at & 15) == 0 && off + g.need <= a.staging_bytes;
-      *ti = -1;
-      if (ROPE && *seen) {
-        *ti = a.rope_idx[p];
-        if (*ti < -1 || *ti >= a.n_tables) *ti = -1;
-      }
-      const rsrc_t r = make_rsrc(static_cast<const uint8_t*>(a.staging) + (*seen ? off : 0),
-                                 *seen ? g.need : 0);
-      const int row = h * a.block_size + (int)(t % a.block_size) + n;
-      const int at_k = row * (Tile::W * 16) + quarter * (Tile::W * 4);
-      load_words<Tile::W>(r, at_k, o->k);
-      load_words<Tile::W>(r, at_k + g.codes, o->v);
-      const int at_s = 2 * g.codes + row * B;
-      const int b0 = B * quarter / 4, b1 = (B * quarter + B - 1) / 4;
-      o->ks[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b0, 0, 0);
-      o->vs[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b0, 0, 0);
-      if constexpr (Tile::S == 2) {
-        o->ks[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b1, 0, 0);
-        o->vs[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b1, 0, 0);
+    // This wave's tokens: a quarter of the stretch. The page tables' entries of 64 pages
+    // lie in the lanes, those of the next 64 are under way.
+    const int per = ((end - begin + kAttendWaves - 1) / kAttendWaves + kStep - 1) / kStep * kStep;
+    const int first = end - begin > wave * per ? begin + wave * per : end;
+    const int last = end - first > per ? first + per : end;
+    int page0 = (int)div_by((uint32_t)first, g.by_block);
+    AttendPages pages = attend_pages<ROPE>(g, rq, page0, lane);
+    AttendPages later = attend_pages<ROPE>(g, rq, page0 + kWave, lane);
+    Tile tile[2];
+    bool seen[2];   // tiles of the step that count
+    int table, step;
+    // the step at t: one tile only where the next one is moved otherwise
+    auto load_step = [&](int t) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const int tt = t + 16 * u;
+        const int p = (int)div_by((uint32_t)tt, g.by_block);
+        if (p - page0 >= kWave) {
+          page0 += kWave;
+          pages = later;
+          later = attend_pages<ROPE>(g, rq, page0 + kWave, lane);
+        }
+        const AttendPage e = page_of<ROPE>(pages, p - page0);
+        seen[u] = tt < last && e.off >= 0;
+        if (u == 0) {
+          table = e.table;
+          step = kStep;
+        } else if (ROPE && e.table != table) {
+          seen[1] = false;
+          step = 16;
+        }
+        const rsrc_t r = make_rsrc(static_cast<const uint8_t*>(a.staging) + (seen[u] ? e.off : 0),
+                                   seen[u] ? g.need : 0);
+        const int row = h * a.block_size + (tt - p * a.block_size) + n;
+        const int at_k = row * (Tile::W * 16) + quarter * (Tile::W * 4);
+        load_words<Tile::W>(r, at_k, tile[u].k);
+        load_words<Tile::W>(r, at_k + g.codes, tile[u].v);
+        const int at_s = 2 * g.codes + row * B;
+        const int b0 = B * quarter / 4, b1 = (B * quarter + B - 1) / 4;
+        tile[u].ks[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b0, 0, 0);
+        tile[u].vs[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b0, 0, 0);
+        if constexpr (Tile::S == 2) {
+          tile[u].ks[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b1, 0, 0);
+          tile[u].vs[1] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + g.scales + b1, 0, 0);
+        }
       }
     };
     // the scale of chunk i of this lane's quarter
@@ -383,66 +448,67 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
       return __any(o);
     };
 
-    for (int64_t t = begin + wave * kStep; t < end; t += kAttendWaves * kStep) {
-      Tile tile[2];
-      bool seen[2];
-      int ti[2];
-      load_tile(t, &tile[0], &seen[0], &ti[0]);
-      load_tile(t + 16, &tile[1], &seen[1], &ti[1]);
-      f32x4 s[NQ][2];
+    int held = -1;  // the table that the queries are rotated by
+    if (first < last) load_step(first);
+    for (int t = first; t < last;) {
+      if (ROPE && table != held) {
+        held = table;
+        const float2* cs = held < 0 ? nullptr : reinterpret_cast<const float2*>(a.cos_sin) +
+                                                    (int64_t)held * (a.rot_dim / 2);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        if (ROPE && seen[u] && ti[u] != table) {
-          table = ti[u];
-          const float2* cs = table < 0 ? nullptr : reinterpret_cast<const float2*>(a.cos_sin) +
-                                                       (int64_t)table * (a.rot_dim / 2);
-#pragma unroll
-          for (int j = 0; j < NQ; ++j)
-            load_query<DT, D, ROPE>(a, qrow[j], quarter, cs, qh[j], ql[j]);
-        }
-#pragma unroll
-        for (int j = 0; j < NQ; ++j) s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        const bool slow = odd(tile[u].ks);
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          const uint32_t* w = tile[u].k + i * (Tile::W / B);
-          const uint32_t sc = scale_of(tile[u].ks, i);
-          u32x4 kf;
-          if (__builtin_expect(slow, 0)) kf = dequantise_saturated<FMT, DT>(w, sc);
-          else kf = dequantise<FMT, DT>(w, sc);
-#pragma unroll
-          for (int j = 0; j < NQ; ++j) {
-            s[j][u] = mfma32<DT>(kf, qh[j][i], s[j][u]);
-            if (ROPE && table >= 0) s[j][u] = mfma32<DT>(kf, ql[j][i], s[j][u]);
-          }
-        }
+        for (int j = 0; j < NQ; ++j)
+          load_query<DT, D, ROPE>(a, qrow[j], quarter, cs, qh[j], ql[j]);
       }
-
-      // V of both tiles to LDS, its NaN blocks as zeros that are put back below
+      // K as operands; V to LDS, its NaN blocks as zeros that are put back below
+      u32x4 kf[2][B];
+      uint32_t nan_scale[2][Tile::S];
       bool any_nan = false;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bool slow = odd(tile[u].vs);
-        const int64_t tok = t + 16 * u + n;
-        const bool row_in = seen[u] && tok < tmax;
+        const bool slow_k = odd(tile[u].ks), slow_v = odd(tile[u].vs);
+        const bool row_in = seen[u] && t + 16 * u + n < tmax;
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          const uint32_t* w = tile[u].v + i * (Tile::W / B);
+          kf[u][i] = dequantise<FMT, DT>(tile[u].k + i * (Tile::W / B), scale_of(tile[u].ks, i));
+          if (__builtin_expect(slow_k, 0)) kf[u][i] = saturate<DT>(kf[u][i], scale_of(tile[u].ks, i));
           const uint32_t sc = scale_of(tile[u].vs, i);
-          u32x4 vf;
-          if (__builtin_expect(slow, 0)) {
-            vf = dequantise_saturated<FMT, DT>(w, sc);
+          u32x4 vf = dequantise<FMT, DT>(tile[u].v + i * (Tile::W / B), sc);
+          if (__builtin_expect(slow_v, 0)) {
+            vf = saturate<DT>(vf, sc);
             if (sc == 255u || !row_in) vf = u32x4{0u, 0u, 0u, 0u};
-          } else {
-            vf = dequantise<FMT, DT>(w, sc);
           }
           mine[lds_place<D>(16 * u + n, quarter * B + i)] = vf;
         }
-        any_nan |= slow;
+        any_nan |= slow_v;
+#pragma unroll
+        for (int i = 0; i < Tile::S; ++i) nan_scale[u][i] = tile[u].vs[i];
+      }
+      const int t0 = t;
+      const bool now[2] = {seen[0], seen[1]};
+      t += step;
+      if (t < last) load_step(t);
+
+      f32x4 s[NQ][2];
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[u][i], qh[j][i], s[j][u]);
+        }
+      }
+      if (ROPE && held >= 0) {
+#pragma unroll
+        for (int j = 0; j < NQ; ++j)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+#pragma unroll
+            for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[u][i], ql[j][i], s[j][u]);
       }
 
       // P
-      const bool masked = t + kStep > tmin || !seen[0] || !seen[1];
+      const bool masked = t0 + kStep > tmin || !now[0] || !now[1];
       u32x4 pf[NQ];
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
@@ -450,19 +516,17 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
         const float base = m[j] == ninf ? 0.0f : m[j];
         float top = ninf;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          x[e] = __builtin_fmaf(s[j][e >> 2][e & 3], g.scale2, -base);
-          if (masked) {
-            const int64_t tok = t + 16 * (e >> 2) + 4 * quarter + (e & 3);
-            if (tok >= lim[j] || !seen[e >> 2]) x[e] = ninf;
-          }
-          top = __builtin_fmaxf(top, x[e]);
+        for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s[j][e >> 2][e & 3], g.scale2, -base);
+        if (masked) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (t0 + 16 * (e >> 2) + 4 * quarter + (e & 3) >= lim[j] || !now[e >> 2]) x[e] = ninf;
         }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = __builtin_fmaxf(top, x[e]);
         if (__any(top > 8.0f || (m[j] == ninf && top > ninf))) {
-          float o = __shfl_xor(top, 16);
-          top = __builtin_fmaxf(top, o);
-          o = __shfl_xor(top, 32);
-          top = __builtin_fmaxf(top, o);
+          top = __builtin_fmaxf(top, __shfl_xor(top, 16));
+          top = __builtin_fmaxf(top, __shfl_xor(top, 32));
           const float mn = __builtin_fmaxf(m[j], top + base);
           if (mn != ninf) {
             const float keep = exp2_(m[j] - mn);
@@ -509,15 +573,15 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
 #pragma unroll
           for (int b = 0; b < B; ++b) {
             // lanes whose quarter begins in block b, or reaches it
-            bool bad = tile[u].vs[0] == 255u && B * quarter / 4 == b;
+            bool bad = nan_scale[u][0] == 255u && B * quarter / 4 == b;
             if constexpr (Tile::S == 2)
-              bad |= tile[u].vs[1] == 255u && (B * quarter + B - 1) / 4 == b;
-            uint64_t rows_nan = __ballot(bad && seen[u]);
+              bad |= nan_scale[u][1] == 255u && (B * quarter + B - 1) / 4 == b;
+            uint64_t rows_nan = __ballot(bad && now[u]);
             rows_nan |= rows_nan >> 32;
             rows_nan |= rows_nan >> 16;
             uint32_t left = (uint32_t)rows_nan & 0xffffu;
             while (left) {
-              const int64_t tok = t + 16 * u + __builtin_ctz(left);
+              const int tok = t0 + 16 * u + __builtin_ctz(left);
               left &= left - 1;
 #pragma unroll
               for (int j = 0; j < NQ; ++j)

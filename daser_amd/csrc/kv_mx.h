@@ -1,7 +1,7 @@
 // kv_mx.h -- quantised records (OCP microscaling formats): the elements' codecs and the
 // kernels that write records from the paged caches and read them back, by page and by
 // token.
-// Part of libdaser_kv: included by kv_mx.hip.
+// Part of libdaser_kv.
 //
 // A block of 32 elements of one (token, head) row is held as q_i 2^(s - 127). With a =
 // max |x_i|, s is the smallest code with a <= T 2^(s - 127), T the format's largest
@@ -19,6 +19,18 @@
 #include "kv_flat.h"
 
 namespace {
+
+inline int64_t pad16(int64_t n) { return (n + 15) / 16 * 16; }
+
+// Section bytes of one half; false for geometries that the format does not take.
+inline bool mx_sections(int format, int block, int heads, int dim, int64_t* codes, int64_t* scales) {
+  if (block <= 0 || heads <= 0 || dim <= 0 || dim % 32) return false;
+  const __int128 elems = (__int128)block * heads * dim;
+  if (elems * 2 > 0x7fffffffLL) return false;  // one buffer descriptor per cache page
+  *codes = pad16((int64_t)elems / (format == DSR_MX_FP4 ? 2 : 1));
+  *scales = pad16((int64_t)elems / 32);
+  return true;
+}
 
 struct MxArgs {
   const uint64_t* layer_base;
