@@ -310,30 +310,34 @@ __device__ __forceinline__ void load_query(const dsr_attend_args& a, const uint8
 constexpr int kAttendWaves = 4;
 constexpr int kStep = 32;  // tokens of a step
 
-// 16-byte chunks of a V row in LDS, and the place of chunk c of row n. Writes put one
-// chunk of 16 rows down together, transposing reads take two neighbouring chunks of 8
-// rows: under this permutation both meet each bank once.
+// Bytes of a V row in LDS: 32 more than it holds, so that 8 rows of two 16-byte chunks (a
+// transposing read of 32 lanes) and 8 rows of one (a write of 8 lanes) meet each bank once,
+// and every address is a lane's base and a constant.
 template <int D>
-__device__ __forceinline__ constexpr int lds_chunks() {
-  return D <= 64 ? 8 : D <= 128 ? 16 : 32;
+__device__ __forceinline__ constexpr int lds_row() {
+  return 2 * D + 32;
 }
-template <int D>
-__device__ __forceinline__ int lds_place(int n, int c) {
-  if constexpr (D <= 64) return n * 8 + (c ^ (((n >> 1) & 3) << 1 | ((n >> 3) & 1)));
-  return n * lds_chunks<D>() + (c ^ ((n & 7) << 1 | ((n >> 3) & 1)));
+
+// Waves per SIMD that the registers are to leave room for.
+template <int D, int NQ, bool ROPE>
+constexpr int attend_waves() {
+  if (NQ == 1) return D <= 64 ? 4 : D <= 128 ? 3 : 2;
+  return D * NQ <= 256 ? 2 : 1;
 }
 
 template <int FMT, int DT, int D, int NQ, bool ROPE>
-__global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
+__global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx_attend_kernel(AttendArgs g) {
   const dsr_attend_args& a = g.a;
   constexpr int B = D / 32, NT = D / 16;
   using Tile = AttendTile<FMT, D>;
-  __shared__ u32x4 lds[kAttendWaves * kStep * lds_chunks<D>()];
+  __shared__ u32x4 lds[kAttendWaves * kStep * lds_row<D>() / 16];
   __shared__ float2 lds_ml[kAttendWaves][16];
   const int lane = (int)threadIdx.x % kWave;
   const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
   const int n = lane & 15, quarter = lane >> 4;
-  u32x4* const mine = lds + wave * kStep * lds_chunks<D>();
+  char* const mine = reinterpret_cast<char*>(lds) + wave * kStep * lds_row<D>();
+  char* const put = mine + n * lds_row<D>() + quarter * (16 * B);
+  char* const get = mine + (4 * quarter + (n >> 2)) * lds_row<D>() + (n & 3) * 8;
   const int h = (int)blockIdx.y;
   const int split = (int)blockIdx.x % g.splits, tile0 = (int)blockIdx.x / g.splits;
   const AttendRequest rq = attend_request(a, (int)blockIdx.z);
@@ -459,25 +463,42 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
         for (int j = 0; j < NQ; ++j)
           load_query<DT, D, ROPE>(a, qrow[j], quarter, cs, qh[j], ql[j]);
       }
-      // K as operands; V to LDS, its NaN blocks as zeros that are put back below
-      u32x4 kf[2][B];
+      // S of each tile; V to LDS, its NaN blocks as zeros that are put back below
+      f32x4 s[NQ][2];
       uint32_t nan_scale[2][Tile::S];
       bool any_nan = false;
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const bool slow_k = odd(tile[u].ks), slow_v = odd(tile[u].vs);
         const bool row_in = seen[u] && t + 16 * u + n < tmax;
+        u32x4 kf[B];
 #pragma unroll
         for (int i = 0; i < B; ++i) {
-          kf[u][i] = dequantise<FMT, DT>(tile[u].k + i * (Tile::W / B), scale_of(tile[u].ks, i));
-          if (__builtin_expect(slow_k, 0)) kf[u][i] = saturate<DT>(kf[u][i], scale_of(tile[u].ks, i));
+          const uint32_t sc = scale_of(tile[u].ks, i);
+          kf[i] = dequantise<FMT, DT>(tile[u].k + i * (Tile::W / B), sc);
+          if (__builtin_expect(slow_k, 0)) kf[i] = saturate<DT>(kf[i], sc);
+        }
+#pragma unroll
+        for (int j = 0; j < NQ; ++j) {
+          s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+          for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[i], qh[j][i], s[j][u]);
+        }
+        if (ROPE && held >= 0) {
+#pragma unroll
+          for (int j = 0; j < NQ; ++j)
+#pragma unroll
+            for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[i], ql[j][i], s[j][u]);
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i) {
           const uint32_t sc = scale_of(tile[u].vs, i);
           u32x4 vf = dequantise<FMT, DT>(tile[u].v + i * (Tile::W / B), sc);
           if (__builtin_expect(slow_v, 0)) {
             vf = saturate<DT>(vf, sc);
             if (sc == 255u || !row_in) vf = u32x4{0u, 0u, 0u, 0u};
           }
-          mine[lds_place<D>(16 * u + n, quarter * B + i)] = vf;
+          *reinterpret_cast<u32x4*>(put + u * (16 * lds_row<D>()) + 16 * i) = vf;
         }
         any_nan |= slow_v;
 #pragma unroll
@@ -487,25 +508,6 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
       const bool now[2] = {seen[0], seen[1]};
       t += step;
       if (t < last) load_step(t);
-
-      f32x4 s[NQ][2];
-#pragma unroll
-      for (int j = 0; j < NQ; ++j) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-          for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[u][i], qh[j][i], s[j][u]);
-        }
-      }
-      if (ROPE && held >= 0) {
-#pragma unroll
-        for (int j = 0; j < NQ; ++j)
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-#pragma unroll
-            for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[u][i], ql[j][i], s[j][u]);
-      }
 
       // P
       const bool masked = t0 + kStep > tmin || !now[0] || !now[1];
@@ -557,10 +559,8 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
         } vt;
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
-          const int row = 16 * u + 4 * quarter + (n >> 2);
-          const int place = lds_place<D>(row, 2 * k + ((n & 3) >> 1)) * 16 + (n & 1) * 8;
           vt.h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(reinterpret_cast<char*>(mine) + place));
+              (__attribute__((address_space(3))) s16x4*)(get + u * (16 * lds_row<D>()) + 32 * k));
         }
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[j][k] = mfma32<DT>(vt.v, pf[j], acc[j][k]);
@@ -645,36 +645,55 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_kernel(AttendArgs g) {
   }
 }
 
-// The splits of a row joined in their order: 16 lanes to a row.
+// The splits of a row joined, in their order: a wave to a row, lane s weighing split s,
+// then each lane summing columns.
 template <int DT>
 __global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs g) {
   const dsr_attend_args& a = g.a;
   const AttendRequest rq = attend_request(a, (int)blockIdx.z);
-  const int sub = (int)threadIdx.x & 15;
-  const int hq = (int)blockIdx.y * (kThreads / 16) + ((int)threadIdx.x >> 4);
+  const int lane = (int)threadIdx.x % kWave;
+  const int hq = __builtin_amdgcn_readfirstlane((int)(blockIdx.y * (kThreads / kWave) +
+                                                      threadIdx.x / kWave));
   if (hq >= a.q_heads) return;
   const float ninf = -__builtin_inff();
   for (int i = rq.q0 + (int)blockIdx.x; i < rq.q1; i += (int)gridDim.x) {
     const int64_t at = (int64_t)i * a.q_heads + hq;
     int64_t seen = rq.tokens;
     if (a.limits && a.limits[i] < seen) seen = a.limits[i];
-    int64_t n = seen <= 0 ? 0 : (seen + g.chunk - 1) / g.chunk;
+    int n = seen <= 0 ? 0 : (int)((seen + g.chunk - 1) / g.chunk);
     if (n > g.splits) n = g.splits;
-    float m = ninf, l = 0.0f;
     const float2* ml = g.part_ml + at * g.splits;
-    for (int s = 0; s < n; ++s) m = __builtin_fmaxf(m, ml[s].x);
-    for (int s = 0; s < n; ++s) l += ml[s].y == 0.0f ? 0.0f : ml[s].y * exp2_(ml[s].x - m);
-    const AttendScale sc = attend_scale(a, at, m, l);
-    if (sub == 0) a.lse[at] = sc.lse;
-    for (int d = sub * 4; d < a.head_dim; d += 64) {
-      f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
-      for (int s = 0; s < n; ++s) {
-        if (ml[s].y == 0.0f) continue;
-        sum += *reinterpret_cast<const f32x4*>(g.part_o + (at * g.splits + s) * a.head_dim + d) *
-               exp2_(ml[s].x - m);
+    const float* po = g.part_o + at * g.splits * a.head_dim;
+    float m = ninf;
+    for (int s = lane; s < n; s += kWave) m = __builtin_fmaxf(m, ml[s].x);
+#pragma unroll
+    for (int k = 1; k < kWave; k <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, k));
+    float l = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int s0 = 0; s0 < n; s0 += kWave) {
+      float w = 0.0f;
+      if (s0 + lane < n) {
+        const float2 x = ml[s0 + lane];
+        if (x.y != 0.0f) {  // NaN too
+          w = exp2_(x.x - m);
+          l += x.y * w;
+        }
       }
-      attend_store<DT>(a, at, d, sum, sc);
+      const int stop = n - s0 < kWave ? n - s0 : kWave;
+      if (lane * 4 < a.head_dim) {
+#pragma unroll 8
+        for (int s = 0; s < stop; ++s) {
+          const float ws = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(w), s));
+          const f32x4 o = *reinterpret_cast<const f32x4*>(po + (int64_t)(s0 + s) * a.head_dim + lane * 4);
+          if (ws != 0.0f) sum += o * ws;
+        }
+      }
     }
+#pragma unroll
+    for (int k = 1; k < kWave; k <<= 1) l += __shfl_xor(l, k);
+    const AttendScale sc = attend_scale(a, at, m, l);
+    if (lane == 0) a.lse[at] = sc.lse;
+    if (lane * 4 < a.head_dim) attend_store<DT>(a, at, lane * 4, sum, sc);
   }
 }
 

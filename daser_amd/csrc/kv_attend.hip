@@ -17,7 +17,9 @@ constexpr int kAttendMinChunk = 128;  // tokens: a step of each wave
 // 16-row column tiles per workgroup.
 int attend_nq(const AttendArgs& g) {
   const int64_t rows = (int64_t)(g.a.max_queries < 1 ? 1 : g.a.max_queries) * g.group;
-  return rows <= 16 ? 1 : g.a.head_dim == 256 ? 2 : 4;
+  const int d = g.a.head_dim;
+  if (rows <= 16 || (d == 256 && g.a.rope_idx)) return 1;
+  return d == 256 || (d >= 96 && g.a.rope_idx) ? 2 : 4;
 }
 
 // The call's geometry checked and its launch planned; *work: there is something to do.
@@ -81,28 +83,29 @@ int64_t attend_bytes(const AttendArgs& g) {
   return attend_ml_bytes(g) + (int64_t)g.a.n_q * g.a.q_heads * g.splits * g.a.head_dim * 4;
 }
 
-template <int FMT, int DT, int D, int NQ>
+template <int FMT, int DT, int D>
 void launch_attend_as(const AttendArgs& g, dim3 grid, hipStream_t s) {
-  if (g.a.rope_idx) kv_mx_attend_kernel<FMT, DT, D, NQ, true><<<grid, kThreads, 0, s>>>(g);
-  else kv_mx_attend_kernel<FMT, DT, D, NQ, false><<<grid, kThreads, 0, s>>>(g);
+  constexpr int kWide = D == 256 ? 2 : 4, kWideRope = D == 256 ? 1 : D >= 96 ? 2 : 4;
+  if (g.a.rope_idx) {
+    if (attend_nq(g) > 1)
+      kv_mx_attend_kernel<FMT, DT, D, kWideRope, true><<<grid, kThreads, 0, s>>>(g);
+    else
+      kv_mx_attend_kernel<FMT, DT, D, 1, true><<<grid, kThreads, 0, s>>>(g);
+  } else {
+    if (attend_nq(g) > 1)
+      kv_mx_attend_kernel<FMT, DT, D, kWide, false><<<grid, kThreads, 0, s>>>(g);
+    else
+      kv_mx_attend_kernel<FMT, DT, D, 1, false><<<grid, kThreads, 0, s>>>(g);
+  }
 }
 template <int FMT, int DT>
 void launch_attend_dims(const AttendArgs& g, dim3 grid, hipStream_t s) {
-  const bool wide = attend_nq(g) > 1;
   switch (g.a.head_dim) {
-#define DSR_ATTEND(D, N)                                          \
-  case D:                                                         \
-    if (wide) launch_attend_as<FMT, DT, D, N>(g, grid, s);        \
-    else launch_attend_as<FMT, DT, D, 1>(g, grid, s);             \
-    break;
-    DSR_ATTEND(32, 4)
-    DSR_ATTEND(64, 4)
-    DSR_ATTEND(96, 4)
-    DSR_ATTEND(128, 4)
-    default:
-      if (wide) launch_attend_as<FMT, DT, 256, 2>(g, grid, s);
-      else launch_attend_as<FMT, DT, 256, 1>(g, grid, s);
-#undef DSR_ATTEND
+    case 32: launch_attend_as<FMT, DT, 32>(g, grid, s); break;
+    case 64: launch_attend_as<FMT, DT, 64>(g, grid, s); break;
+    case 96: launch_attend_as<FMT, DT, 96>(g, grid, s); break;
+    case 128: launch_attend_as<FMT, DT, 128>(g, grid, s); break;
+    default: launch_attend_as<FMT, DT, 256>(g, grid, s);
   }
 }
 void launch_attend(const AttendArgs& g, int n_req, hipStream_t s) {
@@ -117,7 +120,7 @@ void launch_attend(const AttendArgs& g, int n_req, hipStream_t s) {
   }
 }
 void launch_attend_join(const AttendArgs& g, int n_req, hipStream_t s) {
-  const int per = kThreads / 16;
+  const int per = kThreads / kWave;
   const int64_t y = (g.a.q_heads + per - 1) / per;
   const int64_t room = max_wg_per_launch() / (y * n_req);
   int64_t x = g.a.max_queries < 1 ? 1 : g.a.max_queries;
