@@ -31,6 +31,7 @@ struct AttendArgs {
   int32_t group;          // query heads per KV head
   int32_t tiles, splits;  // of blockIdx.x
   int32_t chunk;          // tokens of a split (the last one takes the rest)
+  int32_t wave_heads;     // KV heads of a workgroup: 4 / wave_heads waves share a head's tokens
   float scale2;           // scale * log2(e)
   FastDiv by_block;       // tokens to pages
   float* part_o;          // [n_q * q_heads][splits][head_dim]
@@ -201,7 +202,7 @@ struct AttendTile {
   uint32_t ks[S], vs[S];
 };
 
-template <int W>
+template <int W, int POLICY>
 __device__ __forceinline__ void load_words(rsrc_t r, int off, uint32_t* w) {
   typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
   typedef unsigned int u32x3 __attribute__((ext_vector_type(3)));
@@ -209,7 +210,7 @@ __device__ __forceinline__ void load_words(rsrc_t r, int off, uint32_t* w) {
   if constexpr (W >= 4) {
 #pragma unroll
     for (int k = 0; k < W / 4; ++k, i += 4) {
-      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, 0, 0);
+      const u32x4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * k, 0, POLICY);
       w[i] = x[0];
       w[i + 1] = x[1];
       w[i + 2] = x[2];
@@ -217,14 +218,14 @@ __device__ __forceinline__ void load_words(rsrc_t r, int off, uint32_t* w) {
     }
   }
   constexpr int rest = W % 4, at = W / 4 * 4;
-  if constexpr (rest == 1) w[at] = __builtin_amdgcn_raw_buffer_load_b32(r, off + 4 * at, 0, 0);
+  if constexpr (rest == 1) w[at] = __builtin_amdgcn_raw_buffer_load_b32(r, off + 4 * at, 0, POLICY);
   if constexpr (rest == 2) {
-    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off + 4 * at, 0, 0);
+    const u32x2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off + 4 * at, 0, POLICY);
     w[at] = x[0];
     w[at + 1] = x[1];
   }
   if constexpr (rest == 3) {
-    const u32x3 x = __builtin_amdgcn_raw_buffer_load_b96(r, off + 4 * at, 0, 0);
+    const u32x3 x = __builtin_amdgcn_raw_buffer_load_b96(r, off + 4 * at, 0, POLICY);
     w[at] = x[0];
     w[at + 1] = x[1];
     w[at + 2] = x[2];
@@ -264,51 +265,77 @@ __device__ __forceinline__ AttendPage page_of(const AttendPages& x, int i) {
   return {(int64_t)((uint64_t)hi << 32 | lo), ROPE ? __builtin_amdgcn_readlane(x.table, i) : -1};
 }
 
-// Query rows of this lane's column as MFMA operands: chunk i of quarter g, rotated by
-// -delta with table cs (null: as they are); lo: what the rounding of hi left.
-template <int DT, int D, bool ROPE>
-__device__ __forceinline__ void load_query(const dsr_attend_args& a, const uint8_t* row, int quarter,
-                                           const float2* cs, u32x4* hi, u32x4* lo) {
+// Query rows of this lane's columns as MFMA operands: chunk i of its quarter. Rows that do
+// not exist (bit j of `in` clear) point to one that does and become zeros: without branches
+// the loads go out together.
+template <int D, int NQ>
+__device__ __forceinline__ void load_queries(const uint8_t* const* rows, uint32_t in, int quarter,
+                                             u32x4 (*hi)[D / 32]) {
   constexpr int B = D / 32;
 #pragma unroll
+  for (int j = 0; j < NQ; ++j) {
+    const uint32_t mask = in >> j & 1 ? ~0u : 0u;
+#pragma unroll
+    for (int i = 0; i < B; ++i)
+      hi[j][i] = *reinterpret_cast<const u32x4*>(rows[j] + 16 * (quarter * B + i)) & mask;
+  }
+}
+// One of those rows rotated by -delta with table cs; lo: what the rounding of hi left. The
+// chunks are made in a loop that stays one and pass through `room` (2 KiB a chunk of the
+// wave's LDS, free between steps): unrolled, their values push the accumulators out of the
+// registers (questions over moved chunks 98 -> 133 us).
+template <int DT, int D>
+__device__ __forceinline__ void turn_query(const dsr_attend_args& a, const uint8_t* row, bool in,
+                                           int quarter, const float2* cs, char* room, u32x4* hi,
+                                           u32x4* lo) {
+  constexpr int B = D / 32;
+  const bool neox = a.style == DSR_ROPE_NEOX;
+  const int half = a.rot_dim / 16;  // chunks to the neox partner
+  const uint32_t mask = in ? ~0u : 0u;
+  char* const put = room + (int)(threadIdx.x % kWave) * 16;
+#pragma unroll 1
   for (int i = 0; i < B; ++i) {
     const int c = quarter * B + i;  // 8 elements
-    u32x4 x = row ? *reinterpret_cast<const u32x4*>(row + 16 * c) : u32x4{0u, 0u, 0u, 0u};
-    if constexpr (ROPE) lo[i] = u32x4{0u, 0u, 0u, 0u};
-    if (ROPE && cs && row && c * 8 < a.rot_dim) {
-      const bool neox = a.style == DSR_ROPE_NEOX;
-      const int half = a.rot_dim / 16;  // chunks to the neox partner
-      const bool lower = c < half;
-      const u32x4 y = neox ? *reinterpret_cast<const u32x4*>(row + 16 * (lower ? c + half : c - half))
-                           : x;
-      const float2* t = cs + (neox ? (lower ? c : c - half) * 8 : c * 4);
-      u32x4 h, l;
+    const bool turned = c * 8 < a.rot_dim;
+    const bool lower = c < half;
+    const int pair = !turned ? 0 : neox ? (lower ? c : c - half) * 8 : c * 4;
+    const int partner = !turned || !neox ? c : lower ? c + half : c - half;
+    const f32x4* p = reinterpret_cast<const f32x4*>(cs + pair);
+    // two pairs each: 8 (neox) or 4 (gptj, whose second half is not used) of them
+    const f32x4 t[4] = {p[0], p[1], p[neox ? 2 : 0], p[neox ? 3 : 1]};
+    const float flip = neox && !lower ? -1.0f : 1.0f;
+    const u32x4 x = *reinterpret_cast<const u32x4*>(row + 16 * c) & mask;
+    const u32x4 y = *reinterpret_cast<const u32x4*>(row + 16 * partner) & mask;
+    u32x4 h, l;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float x0 = half_of<DT>(x[k], 0), x1 = half_of<DT>(x[k], 1);
-        float r0, r1;
-        if (neox) {
-          const float2 t0 = t[2 * k], t1 = t[2 * k + 1];
-          const float y0 = half_of<DT>(y[k], 0), y1 = half_of<DT>(y[k], 1);
-          r0 = lower ? x0 * t0.x + y0 * t0.y : x0 * t0.x - y0 * t0.y;
-          r1 = lower ? x1 * t1.x + y1 * t1.y : x1 * t1.x - y1 * t1.y;
-        } else {
-          const float2 t0 = t[k];
-          r0 = x0 * t0.x + x1 * t0.y;
-          r1 = x1 * t0.x - x0 * t0.y;
-        }
-        h[k] = pack2<DT>(r0, r1);
-        l[k] = pack2<DT>(r0 - half_of<DT>(h[k], 0), r1 - half_of<DT>(h[k], 1));
-      }
-      x = h;
-      lo[i] = l;
+    for (int k = 0; k < 4; ++k) {
+      const float x0 = half_of<DT>(x[k], 0), x1 = half_of<DT>(x[k], 1);
+      // neox: pairs (2 k, 2 k + 1) with the partner's; gptj: pair k with itself
+      const float y0 = neox ? half_of<DT>(y[k], 0) : x1, y1 = neox ? half_of<DT>(y[k], 1) : -x0;
+      const float c0 = neox ? t[k][0] : t[k >> 1][2 * (k & 1)];
+      const float s0 = neox ? t[k][1] : t[k >> 1][2 * (k & 1) + 1];
+      const float c1 = neox ? t[k][2] : c0, s1 = neox ? t[k][3] : s0;
+      const float r0 = turned ? x0 * c0 + y0 * (flip * s0) : x0;
+      const float r1 = turned ? x1 * c1 + y1 * (flip * s1) : x1;
+      h[k] = pack2<DT>(r0, r1);
+      l[k] = pack2<DT>(r0 - half_of<DT>(h[k], 0), r1 - half_of<DT>(h[k], 1));
     }
-    hi[i] = x;
+    *reinterpret_cast<u32x4*>(put + i * 2048) = h;
+    *reinterpret_cast<u32x4*>(put + i * 2048 + 1024) = l;
+  }
+#pragma unroll
+  for (int i = 0; i < B; ++i) {
+    hi[i] = *reinterpret_cast<const u32x4*>(put + i * 2048);
+    lo[i] = *reinterpret_cast<const u32x4*>(put + i * 2048 + 1024);
   }
 }
 
+// The scheduler moves nothing past it: what it would fetch early costs registers.
+__device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
+
 constexpr int kAttendWaves = 4;
 constexpr int kStep = 32;  // tokens of a step
+
 
 // Bytes of a V row in LDS: 32 more than it holds, so that 8 rows of two 16-byte chunks (a
 // transposing read of 32 lanes) and 8 rows of one (a write of 8 lanes) meet each bank once,
@@ -338,33 +365,36 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
   char* const mine = reinterpret_cast<char*>(lds) + wave * kStep * lds_row<D>();
   char* const put = mine + n * lds_row<D>() + quarter * (16 * B);
   char* const get = mine + (4 * quarter + (n >> 2)) * lds_row<D>() + (n & 3) * 8;
-  const int h = (int)blockIdx.y;
+  const int h = (int)blockIdx.y * g.wave_heads + wave % g.wave_heads;
+  const int share = kAttendWaves / g.wave_heads;  // waves of a head
   const int split = (int)blockIdx.x % g.splits, tile0 = (int)blockIdx.x / g.splits;
   const AttendRequest rq = attend_request(a, (int)blockIdx.z);
   const int64_t rows = rq.q1 > rq.q0 ? (int64_t)(rq.q1 - rq.q0) * g.group : 0;
   const float ninf = -__builtin_inff();
+  auto out_row = [&](int64_t row, int head) {
+    return (int64_t)(rq.q0 + (int)(row / g.group)) * a.q_heads + head * g.group + (int)(row % g.group);
+  };
 
   for (int64_t row0 = (int64_t)tile0 * (16 * NQ); row0 < rows; row0 += (int64_t)g.tiles * (16 * NQ)) {
     // this lane's columns
     int lim[NQ];
     const uint8_t* qrow[NQ];
+    uint32_t in = 0;  // bit j: the column's row exists
     int tmax = 0, tmin = 0x7fffffff;
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
-      const int64_t row = row0 + 16 * j + n;
-      const bool in = row < rows;
-      const int i = rq.q0 + (int)(row / g.group);
-      lim[j] = 0;
-      qrow[j] = nullptr;
-      if (in) {
-        int64_t seen = rq.tokens;
-        if (a.limits && a.limits[i] < seen) seen = a.limits[i];
-        lim[j] = seen < 0 ? 0 : (int)seen;
-        qrow[j] = static_cast<const uint8_t*>(a.q) + (int64_t)i * a.q_row_stride +
-                  (int64_t)(h * g.group + (int)(row % g.group)) * a.q_head_stride;
-        tmin = lim[j] < tmin ? lim[j] : tmin;
-      }
-      tmax = lim[j] > tmax ? lim[j] : tmax;
+      const int64_t row = row0 + 16 * j + n < rows ? row0 + 16 * j + n : rows - 1;
+      const bool is = row0 + 16 * j + n < rows;
+      const int i = rq.q0 + (int)((uint32_t)row / (uint32_t)g.group);
+      const int hq = (int)((uint32_t)row % (uint32_t)g.group);
+      int64_t seen = rq.tokens;
+      if (a.limits && a.limits[i] < seen) seen = a.limits[i];
+      lim[j] = !is || seen < 0 ? 0 : (int)seen;
+      if (is && lim[j] < tmin) tmin = lim[j];
+      if (lim[j] > tmax) tmax = lim[j];
+      in |= (uint32_t)is << j;
+      qrow[j] = static_cast<const uint8_t*>(a.q) + (int64_t)i * a.q_row_stride +
+                (int64_t)(h * g.group + hq) * a.q_head_stride;
     }
 #pragma unroll
     for (int k = 1; k < 16; k <<= 1) {
@@ -381,9 +411,12 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
     if (begin >= end && split > 0) continue;  // the join does not read it
 
     u32x4 qh[NQ][B], ql[ROPE ? NQ : 1][ROPE ? B : 1];
+    load_queries<D, NQ>(qrow, in, quarter, qh);
+    if constexpr (ROPE)
 #pragma unroll
-    for (int j = 0; j < NQ; ++j)
-      load_query<DT, D, ROPE>(a, qrow[j], quarter, nullptr, qh[j], ql[ROPE ? j : 0]);
+      for (int j = 0; j < NQ; ++j)
+#pragma unroll
+        for (int i = 0; i < B; ++i) ql[j][i] = u32x4{0u, 0u, 0u, 0u};
     f32x4 acc[NQ][NT];
     float m[NQ], l[NQ];
 #pragma unroll
@@ -394,43 +427,53 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
       for (int t = 0; t < NT; ++t) acc[j][t] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    // This wave's tokens: a quarter of the stretch. The page tables' entries of 64 pages
+    // This wave's tokens: its share of the stretch. The page tables' entries of 64 pages
     // lie in the lanes, those of the next 64 are under way.
-    const int per = ((end - begin + kAttendWaves - 1) / kAttendWaves + kStep - 1) / kStep * kStep;
-    const int first = end - begin > wave * per ? begin + wave * per : end;
+    const int per = ((end - begin + share - 1) / share + kStep - 1) / kStep * kStep;
+    const int turn = wave / g.wave_heads;
+    const int first = end - begin > turn * per ? begin + turn * per : end;
     const int last = end - first > per ? first + per : end;
     int page0 = (int)div_by((uint32_t)first, g.by_block);
     AttendPages pages = attend_pages<ROPE>(g, rq, page0, lane);
     AttendPages later = attend_pages<ROPE>(g, rq, page0 + kWave, lane);
+    // The step whose loads are under way: its tiles, which of them count, its first token, its
+    // table. (Two steps ahead cost the registers of a third wave: decode batch 174 -> 198 us.)
     Tile tile[2];
-    bool seen[2];   // tiles of the step that count
-    int table, step;
-    // the step at t: one tile only where the next one is moved otherwise
-    auto load_step = [&](int t) {
+    bool seen[2];
+    int at, turned;
+    int next = first;
+    // the step at t: one tile only where the next one is moved otherwise, or its page's
+    // entry is not in the lanes yet
+    auto load_step = [&]() {
+      const int t = next;
+      at = t;
+      if (t >= last) return;
+      if ((int)div_by((uint32_t)t, g.by_block) - page0 >= kWave) {
+        page0 += kWave;
+        pages = later;
+        later = attend_pages<ROPE>(g, rq, page0 + kWave, lane);
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
         const int tt = t + 16 * u;
         const int p = (int)div_by((uint32_t)tt, g.by_block);
-        if (p - page0 >= kWave) {
-          page0 += kWave;
-          pages = later;
-          later = attend_pages<ROPE>(g, rq, page0 + kWave, lane);
-        }
-        const AttendPage e = page_of<ROPE>(pages, p - page0);
+        const AttendPage e = page_of<ROPE>(pages, (p - page0) & (kWave - 1));
         seen[u] = tt < last && e.off >= 0;
         if (u == 0) {
-          table = e.table;
-          step = kStep;
-        } else if (ROPE && e.table != table) {
+          turned = e.table;
+          next = t + kStep;
+        } else if (p - page0 >= kWave || (ROPE && e.table != turned)) {
           seen[1] = false;
-          step = 16;
+          next = t + 16;
         }
         const rsrc_t r = make_rsrc(static_cast<const uint8_t*>(a.staging) + (seen[u] ? e.off : 0),
                                    seen[u] ? g.need : 0);
         const int row = h * a.block_size + (tt - p * a.block_size) + n;
         const int at_k = row * (Tile::W * 16) + quarter * (Tile::W * 4);
-        load_words<Tile::W>(r, at_k, tile[u].k);
-        load_words<Tile::W>(r, at_k + g.codes, tile[u].v);
+        // one tile of rows reads them once: they stream through
+        constexpr int kPolicy = NQ == 1 ? kLoadPolicy : 0;
+        load_words<Tile::W, kPolicy>(r, at_k, tile[u].k);
+        load_words<Tile::W, kPolicy>(r, at_k + g.codes, tile[u].v);
         const int at_s = 2 * g.codes + row * B;
         const int b0 = B * quarter / 4, b1 = (B * quarter + B - 1) / 4;
         tile[u].ks[0] = (uint8_t)__builtin_amdgcn_raw_buffer_load_b8(r, at_s + b0, 0, 0);
@@ -446,71 +489,91 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
       if constexpr (Tile::S == 1) return s[0];
       return (B * quarter + i) / 4 == B * quarter / 4 ? s[0] : s[1];
     };
-    auto odd = [&](const uint32_t* s) -> bool {
-      bool o = s[0] > top_scale<FMT, DT>();
-      if constexpr (Tile::S == 2) o |= s[1] > top_scale<FMT, DT>();
-      return __any(o);
-    };
-
+    // One step on the loaded tiles. odd: scales near the type's largest value or NaN;
+    // masked: tokens that some query does not see, or a tile missing. Both are rare and the
+    // same for the wave.
     int held = -1;  // the table that the queries are rotated by
-    if (first < last) load_step(first);
-    for (int t = first; t < last;) {
-      if (ROPE && table != held) {
-        held = table;
-        const float2* cs = held < 0 ? nullptr : reinterpret_cast<const float2*>(a.cos_sin) +
-                                                    (int64_t)held * (a.rot_dim / 2);
+    auto run_step = [&]() {
+      const int t0 = at;
+      const bool now[2] = {seen[0], seen[1]};
+      if constexpr (ROPE) {
+        if (turned != held) {
+          held = turned;
+          if (held >= 0) {
+            const float2* cs =
+                reinterpret_cast<const float2*>(a.cos_sin) + (int64_t)held * (a.rot_dim / 2);
 #pragma unroll
-        for (int j = 0; j < NQ; ++j)
-          load_query<DT, D, ROPE>(a, qrow[j], quarter, cs, qh[j], ql[j]);
+            for (int j = 0; j < NQ; ++j) {
+              turn_query<DT, D>(a, qrow[j], in >> j & 1, quarter, cs, mine, qh[j], ql[j]);
+              phase();
+            }
+          } else {
+            load_queries<D, NQ>(qrow, in, quarter, qh);
+#pragma unroll
+            for (int j = 0; j < NQ; ++j)
+#pragma unroll
+              for (int i = 0; i < B; ++i) ql[j][i] = u32x4{0u, 0u, 0u, 0u};
+          }
+        }
       }
-      // S of each tile; V to LDS, its NaN blocks as zeros that are put back below
+      bool odd = false;
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int i = 0; i < Tile::S; ++i)
+          odd |= tile[u].ks[i] > top_scale<FMT, DT>() || tile[u].vs[i] > top_scale<FMT, DT>();
+      odd = __any(odd);
+      const bool masked = t0 + kStep > tmin || !now[0] || !now[1];
       f32x4 s[NQ][2];
       uint32_t nan_scale[2][Tile::S];
-      bool any_nan = false;
+      // S of each tile; V to LDS, its NaN blocks as zeros that are put back below
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
-        const bool slow_k = odd(tile[u].ks), slow_v = odd(tile[u].vs);
-        const bool row_in = seen[u] && t + 16 * u + n < tmax;
+        const bool row_in = now[u] && t0 + 16 * u + n < tmax;
+        u32x4 vf[B];
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          vf[i] = dequantise<FMT, DT>(tile[u].v + i * (Tile::W / B), scale_of(tile[u].vs, i));
+        if (__builtin_expect(odd, 0)) {
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const uint32_t sv = scale_of(tile[u].vs, i);
+            if (sv > top_scale<FMT, DT>()) vf[i] = saturate<DT>(vf[i], sv);
+            if (sv == 255u || !row_in) vf[i] = u32x4{0u, 0u, 0u, 0u};
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < B; ++i)
+          *reinterpret_cast<u32x4*>(put + u * (16 * lds_row<D>()) + 16 * i) = vf[i];
+        phase();
         u32x4 kf[B];
 #pragma unroll
-        for (int i = 0; i < B; ++i) {
-          const uint32_t sc = scale_of(tile[u].ks, i);
-          kf[i] = dequantise<FMT, DT>(tile[u].k + i * (Tile::W / B), sc);
-          if (__builtin_expect(slow_k, 0)) kf[i] = saturate<DT>(kf[i], sc);
+        for (int i = 0; i < B; ++i)
+          kf[i] = dequantise<FMT, DT>(tile[u].k + i * (Tile::W / B), scale_of(tile[u].ks, i));
+        if (__builtin_expect(odd, 0)) {
+#pragma unroll
+          for (int i = 0; i < B; ++i) {
+            const uint32_t sk = scale_of(tile[u].ks, i);
+            if (sk > top_scale<FMT, DT>()) kf[i] = saturate<DT>(kf[i], sk);
+          }
         }
 #pragma unroll
         for (int j = 0; j < NQ; ++j) {
           s[j][u] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-          for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[i], qh[j][i], s[j][u]);
-        }
-        if (ROPE && held >= 0) {
-#pragma unroll
-          for (int j = 0; j < NQ; ++j)
-#pragma unroll
-            for (int i = 0; i < B; ++i) s[j][u] = mfma32<DT>(kf[i], ql[j][i], s[j][u]);
-        }
-#pragma unroll
-        for (int i = 0; i < B; ++i) {
-          const uint32_t sc = scale_of(tile[u].vs, i);
-          u32x4 vf = dequantise<FMT, DT>(tile[u].v + i * (Tile::W / B), sc);
-          if (__builtin_expect(slow_v, 0)) {
-            vf = saturate<DT>(vf, sc);
-            if (sc == 255u || !row_in) vf = u32x4{0u, 0u, 0u, 0u};
+          for (int i = 0; i < B; ++i) {
+            s[j][u] = mfma32<DT>(kf[i], qh[j][i], s[j][u]);
+            if (ROPE) s[j][u] = mfma32<DT>(kf[i], ql[j][i], s[j][u]);
           }
-          *reinterpret_cast<u32x4*>(put + u * (16 * lds_row<D>()) + 16 * i) = vf;
         }
-        any_nan |= slow_v;
 #pragma unroll
         for (int i = 0; i < Tile::S; ++i) nan_scale[u][i] = tile[u].vs[i];
+        phase();
       }
-      const int t0 = t;
-      const bool now[2] = {seen[0], seen[1]};
-      t += step;
-      if (t < last) load_step(t);
+      load_step();
+      phase();
 
       // P
-      const bool masked = t0 + kStep > tmin || !now[0] || !now[1];
       u32x4 pf[NQ];
 #pragma unroll
       for (int j = 0; j < NQ; ++j) {
@@ -518,8 +581,10 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
         const float base = m[j] == ninf ? 0.0f : m[j];
         float top = ninf;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] = __builtin_fmaf(s[j][e >> 2][e & 3], g.scale2, -base);
-        if (masked) {
+        for (int e = 0; e < 8; ++e) {
+          x[e] = __builtin_fmaf(s[j][e >> 2][e & 3], g.scale2, -base);
+        }
+        if (__builtin_expect(masked, 0)) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             if (t0 + 16 * (e >> 2) + 4 * quarter + (e & 3) >= lim[j] || !now[e >> 2]) x[e] = ninf;
@@ -548,6 +613,7 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
         }
 #pragma unroll
         for (int k = 0; k < 4; ++k) pf[j][k] = pack2<DT>(x[2 * k], x[2 * k + 1]);
+        phase();
       }
 
       // O^T: lanes' columns 4 c ... of rows 4 quarter + r, transposed in 16-lane groups
@@ -558,15 +624,14 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
           u32x4 v;
         } vt;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < 2; ++u)
           vt.h[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
               (__attribute__((address_space(3))) s16x4*)(get + u * (16 * lds_row<D>()) + 32 * k));
-        }
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[j][k] = mfma32<DT>(vt.v, pf[j], acc[j][k]);
       }
 
-      if (__builtin_expect(any_nan, 0)) {
+      if (__builtin_expect(odd, 0)) {
         const float nan = __uint_as_float(0x7fc00000u);
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -593,9 +658,36 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
           }
         }
       }
-    }
+    };
 
-    // the 4 waves joined, 16 rows at a time
+    load_step();
+    while (at < last) run_step();
+
+    if (share == 1) {  // every wave has heads of its own: straight from the registers
+#pragma unroll
+      for (int j = 0; j < NQ; ++j) {
+        l[j] += __shfl_xor(l[j], 16);
+        l[j] += __shfl_xor(l[j], 32);
+        const int64_t row = row0 + 16 * j + n;
+        if (row >= rows) continue;
+        const int64_t o = out_row(row, h);
+        AttendScale sc{};
+        if (g.splits == 1) {
+          sc = attend_scale(a, o, m[j], l[j]);
+          if (quarter == 0) a.lse[o] = sc.lse;
+        } else if (quarter == 0) {
+          g.part_ml[o * g.splits + split] = float2{m[j], l[j]};
+        }
+#pragma unroll
+        for (int k = 0; k < NT; ++k) {
+          const int d = 16 * k + 4 * quarter;
+          if (g.splits == 1) attend_store<DT>(a, o, d, acc[j][k], sc);
+          else *reinterpret_cast<f32x4*>(g.part_o + (o * g.splits + split) * D + d) = acc[j][k];
+        }
+      }
+      continue;
+    }
+    // the waves of a head joined, 16 rows at a time
 #pragma unroll
     for (int j = 0; j < NQ; ++j) {
       l[j] += __shfl_xor(l[j], 16);
@@ -610,34 +702,36 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
       const int col = (int)threadIdx.x >> 4;
       const int64_t row = row0 + 16 * j + col;
       if (row < rows) {
-        float mt = ninf, lt = 0.0f, f[kAttendWaves];
+        for (int hh = 0; hh < g.wave_heads; ++hh) {
+          float mt = ninf, lt = 0.0f, f[kAttendWaves];
 #pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) mt = __builtin_fmaxf(mt, lds_ml[w][col].x);
-#pragma unroll
-        for (int w = 0; w < kAttendWaves; ++w) {
-          const float2 ml = lds_ml[w][col];
-          f[w] = ml.y == 0.0f ? 0.0f : exp2_(ml.x - mt);
-          lt += ml.y * f[w];
-        }
-        const int i = rq.q0 + (int)(row / g.group);
-        const int64_t at = (int64_t)i * a.q_heads + h * g.group + (int)(row % g.group);
-        AttendScale sc{};
-        if (g.splits == 1) {
-          sc = attend_scale(a, at, mt, lt);
-          if ((threadIdx.x & 15) == 0) a.lse[at] = sc.lse;
-        } else if ((threadIdx.x & 15) == 0) {
-          g.part_ml[at * g.splits + split] = float2{mt, lt};
-        }
-        for (int d = ((int)threadIdx.x & 15) * 4; d < D; d += 64) {
-          f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+          for (int w = 0; w < kAttendWaves; ++w)
+            if (w % g.wave_heads == hh) mt = __builtin_fmaxf(mt, lds_ml[w][col].x);
 #pragma unroll
           for (int w = 0; w < kAttendWaves; ++w) {
-            const f32x4 x = *reinterpret_cast<const f32x4*>(
-                reinterpret_cast<const float*>(lds) + w * (D * 16) + col * D + (d ^ ((col & 7) << 2)));
-            sum += x * f[w];
+            const float2 ml = lds_ml[w][col];
+            f[w] = w % g.wave_heads != hh || ml.y == 0.0f ? 0.0f : exp2_(ml.x - mt);
+            if (w % g.wave_heads == hh) lt += ml.y * f[w];
           }
-          if (g.splits == 1) attend_store<DT>(a, at, d, sum, sc);
-          else *reinterpret_cast<f32x4*>(g.part_o + (at * g.splits + split) * D + d) = sum;
+          const int64_t o = out_row(row, (int)blockIdx.y * g.wave_heads + hh);
+          AttendScale sc{};
+          if (g.splits == 1) {
+            sc = attend_scale(a, o, mt, lt);
+            if ((threadIdx.x & 15) == 0) a.lse[o] = sc.lse;
+          } else if ((threadIdx.x & 15) == 0) {
+            g.part_ml[o * g.splits + split] = float2{mt, lt};
+          }
+          for (int d = ((int)threadIdx.x & 15) * 4; d < D; d += 64) {
+            f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int w = 0; w < kAttendWaves; ++w)
+              if (w % g.wave_heads == hh)
+                sum += *reinterpret_cast<const f32x4*>(reinterpret_cast<const float*>(lds) +
+                                                       w * (D * 16) + col * D +
+                                                       (d ^ ((col & 7) << 2))) * f[w];
+            if (g.splits == 1) attend_store<DT>(a, o, d, sum, sc);
+            else *reinterpret_cast<f32x4*>(g.part_o + (o * g.splits + split) * D + d) = sum;
+          }
         }
       }
     }
@@ -685,7 +779,7 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs 
         for (int s = 0; s < stop; ++s) {
           const float ws = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(w), s));
           const f32x4 o = *reinterpret_cast<const f32x4*>(po + (int64_t)(s0 + s) * a.head_dim + lane * 4);
-          if (ws != 0.0f) sum += o * ws;
+          sum += o * ws;
         }
       }
     }

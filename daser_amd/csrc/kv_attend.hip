@@ -11,7 +11,9 @@ namespace {
 
 constexpr int kMaxGridZ = 65535;
 
-constexpr int kAttendWgs = 1024;      // workgroups that fill the chip
+constexpr int kAttendWgs = 2048;      // workgroups that fill the chip
+constexpr int kAttendWideWgs = 512;  // of several tiles of rows: two to a CU
+constexpr int64_t kAttendLarge = 256 * 16 * 64;
 constexpr int kAttendMinChunk = 128;  // tokens: a step of each wave
 
 // 16-row column tiles per workgroup.
@@ -62,11 +64,15 @@ int attend_args(const dsr_attend_args* args, AttendArgs* g, bool* work) {
   int64_t tiles = (rows + 16 * nq - 1) / (16 * nq);
   const int64_t nz = a.n_req < kMaxGridZ ? a.n_req : kMaxGridZ;
   const int64_t ctx = a.max_context < 1 ? 1 : a.max_context;
-  int64_t splits = (kAttendWgs + tiles * a.kv_heads * nz - 1) / (tiles * a.kv_heads * nz);
-  const int64_t most = (ctx + kAttendMinChunk - 1) / kAttendMinChunk;
+  g->wave_heads = 1;
+  if (nq == 1 && nz * a.kv_heads * ctx >= kAttendLarge)
+    g->wave_heads = a.kv_heads % 4 == 0 ? 4 : a.kv_heads % 2 == 0 ? 2 : 1;
+  const int64_t least = kAttendMinChunk / g->wave_heads;
+  const int64_t wgs = tiles * (a.kv_heads / g->wave_heads) * nz;
+  int64_t splits = ((nq == 1 ? kAttendWgs : kAttendWideWgs) + wgs - 1) / wgs;
+  const int64_t most = (ctx + least - 1) / least;
   if (splits > most) splits = most;
-  const int64_t chunk = ((ctx + splits - 1) / splits + kAttendMinChunk - 1) / kAttendMinChunk *
-                        kAttendMinChunk;
+  const int64_t chunk = ((ctx + splits - 1) / splits + least - 1) / least * least;
   g->chunk = (int)(chunk < 0x40000000 ? chunk : 0x40000000);
   g->splits = (int)((ctx + g->chunk - 1) / g->chunk);
   // requests larger than the hints loop
@@ -109,7 +115,7 @@ void launch_attend_dims(const AttendArgs& g, dim3 grid, hipStream_t s) {
   }
 }
 void launch_attend(const AttendArgs& g, int n_req, hipStream_t s) {
-  const dim3 grid((unsigned)(g.tiles * g.splits), (unsigned)g.a.kv_heads, (unsigned)n_req);
+  const dim3 grid((unsigned)(g.tiles * g.splits), (unsigned)(g.a.kv_heads / g.wave_heads), (unsigned)n_req);
   const bool bf16 = g.a.dtype == DSR_DTYPE_BF16;
   if (g.a.format == DSR_MX_FP4) {
     if (bf16) launch_attend_dims<DSR_MX_FP4, DSR_DTYPE_BF16>(g, grid, s);
@@ -154,7 +160,7 @@ int dsr_attend_mx(const dsr_attend_args* args, dsr_stream_t stream) {
     return DSR_ERR_ARG;
   if (!aligned16(a.q_row_stride) || !aligned16(a.q_head_stride) || !aligned16p(a.q) ||
       !aligned16p(a.out) || !aligned16p(a.prior_out) || !aligned16p(a.staging) ||
-      !aligned16(a.layer_bytes) || !aligned16p(a.workspace))
+      !aligned16(a.layer_bytes) || !aligned16p(a.workspace) || !aligned16p(a.cos_sin))
     return DSR_ERR_ALIGN;
   const int64_t need = attend_bytes(g);
   if (need > a.workspace_bytes || (need > 0 && !a.workspace)) return DSR_ERR_ARG;
