@@ -75,7 +75,6 @@ constexpr float kLn2 = 0.69314718055994531f;
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
 template <int DT>
@@ -88,72 +87,10 @@ __device__ __forceinline__ f32x4 mfma32(u32x4 a, u32x4 b, f32x4 c) {
                                                   __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// Two floats as q's type, round to nearest even.
-template <int DT>
-__device__ __forceinline__ uint32_t pack2(float x, float y) {
-  const f32x2 f = {x, y};
-  if constexpr (DT == DSR_DTYPE_BF16)
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
-}
 template <int DT>
 __device__ __forceinline__ float half_of(uint32_t w, int k) {
   const uint32_t h = k ? w >> 16 : w & 0xffffu;
   return DT == DSR_DTYPE_BF16 ? bf16_to_f32(h) : fp16_to_f32(h);
-}
-
-// Scale codes above it may read as more than q's type holds (and 255 as NaN): such blocks
-// take the path that saturates.
-template <int FMT, int DT>
-__device__ __forceinline__ constexpr uint32_t top_scale() {
-  return DT == DSR_DTYPE_BF16 ? (FMT == DSR_MX_FP4 ? 252u : 254u)
-                              : (FMT == DSR_MX_FP4 ? 140u : 142u);
-}
-
-// 8 codes (w[0], and w[1] of int8) under scale code s as 8 values of q's type.
-template <int FMT, int DT>
-__device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
-  u32x4 o;
-  if constexpr (FMT == DSR_MX_FP4) {
-    const float scale = mx_scale(s);
-#define DSR_DQ(K)                                                                            \
-  if constexpr (DT == DSR_DTYPE_BF16)                                                        \
-    o[K] = __builtin_bit_cast(uint32_t,                                                      \
-                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, K));    \
-  else                                                                                       \
-    o[K] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], scale, K));
-    DSR_DQ(0)
-    DSR_DQ(1)
-    DSR_DQ(2)
-    DSR_DQ(3)
-#undef DSR_DQ
-  } else {
-    const int e = (int)s - 133;
-    // small scales are subnormal themselves: the power is applied in two steps
-    const float lo = __builtin_ldexpf(1.0f, e < -100 ? e + 64 : e);
-    const float hi = e < -100 ? 0x1p-64f : 1.0f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const uint32_t x = w[k >> 1] >> (16 * (k & 1));
-      o[k] = pack2<DT>((float)(int8_t)x * lo * hi, (float)(int8_t)(x >> 8) * lo * hi);
-    }
-  }
-  return o;
-}
-// The same for blocks above top_scale(): saturated; NaN under 255.
-template <int DT>
-__device__ __forceinline__ u32x4 saturate(u32x4 v, uint32_t s) {
-  constexpr uint32_t top = DT == DSR_DTYPE_BF16 ? 0x7f7f7f7fu : 0x7bff7bffu;
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const uint32_t mag = v[k] & 0x7fff7fffu;
-    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, mag),
-                                              __builtin_bit_cast(u16x2, top));
-    v[k] = s == 255u ? (DT == DSR_DTYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u)
-                     : (v[k] & 0x80008000u) | __builtin_bit_cast(uint32_t, m);
-  }
-  return v;
 }
 
 // out[i][h] and its lse from the unnormalised sum o (4 consecutive columns from d on),
@@ -538,7 +475,8 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
 #pragma unroll
           for (int i = 0; i < B; ++i) {
             const uint32_t sv = scale_of(tile[u].vs, i);
-            if (sv > top_scale<FMT, DT>()) vf[i] = saturate<DT>(vf[i], sv);
+            if (sv > top_scale<FMT, DT>())
+              vf[i] = dequantise_any<FMT, DT>(tile[u].v + i * (Tile::W / B), sv);
             if (sv == 255u || !row_in) vf[i] = u32x4{0u, 0u, 0u, 0u};
           }
         }
@@ -554,7 +492,8 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
 #pragma unroll
           for (int i = 0; i < B; ++i) {
             const uint32_t sk = scale_of(tile[u].ks, i);
-            if (sk > top_scale<FMT, DT>()) kf[i] = saturate<DT>(kf[i], sk);
+            if (sk > top_scale<FMT, DT>())
+              kf[i] = dequantise_any<FMT, DT>(tile[u].k + i * (Tile::W / B), sk);
           }
         }
 #pragma unroll

@@ -76,6 +76,7 @@ __device__ __forceinline__ float mx_scale(uint32_t s) {
 
 typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 // fp32 bits of the largest magnitude of the 4 lanes' 8 elements each (one block);
 // 0x7F800000 and up: one of them is not finite.
@@ -151,31 +152,107 @@ __device__ __forceinline__ void mx_decode(uint2 c, uint32_t s, float* x) {
       x[2 * k + 1] = f[k].y;
     }
   } else {
+    const float p = __builtin_ldexpf(1.0f, (int)s - 133), bias = -128.0f * p;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      const uint32_t w = e < 4 ? c.x : c.y;
-      x[e] = __builtin_ldexpf((float)(int8_t)(w >> (8 * (e & 3))), (int)s - 133);
+      const uint32_t u = (e < 4 ? c.x : c.y) ^ 0x80808080u;
+      x[e] = __builtin_fmaf((float)(u >> (8 * (e & 3)) & 255u), p, bias);
     }
   }
-  if (s == 255u) {
+  if (__builtin_expect(s >= 254u, 0)) {  // 128 p is past fp32, and 255 is NaN
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = __uint_as_float(0x7fc00000u);
+    for (int e = 0; e < 8; ++e) {
+      if (FMT == DSR_MX_INT8)
+        x[e] = __builtin_ldexpf((float)(int8_t)((e < 4 ? c.x : c.y) >> (8 * (e & 3))), (int)s - 133);
+      if (s == 255u) x[e] = __uint_as_float(0x7fc00000u);
+    }
   }
 }
 
-// 8 values as a cache vector: saturated to the type's largest, NaN kept.
+// Scale codes above it may read as more than the type holds, and 255 as NaN.
+template <int FMT, int DT>
+__device__ __forceinline__ constexpr uint32_t top_scale() {
+  return DT == DSR_DTYPE_BF16 ? (FMT == DSR_MX_FP4 ? 252u : 253u)
+                              : (FMT == DSR_MX_FP4 ? 140u : 141u);
+}
+
+// Two floats as the type, round to nearest even.
 template <int DT>
-__device__ __forceinline__ u32x4 mx_store_vec(float* y) {
-  const float top = DT == DSR_DTYPE_BF16 ? __uint_as_float(0x7f7f0000u) : 65504.0f;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    y[e] = y[e] > top ? top : y[e];
-    y[e] = y[e] < -top ? -top : y[e];
-  }
-  u32x4 v;
-  if constexpr (DT == DSR_DTYPE_BF16) {
-    if (Codec<DT>::encode_quick(y, &v)) v = Codec<DT>::encode(y);
+__device__ __forceinline__ uint32_t pack2(float x, float y) {
+  const f32x2 f = {x, y};
+  if constexpr (DT == DSR_DTYPE_BF16)
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, bf16x2));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, f16x2));
+}
+
+// 8 codes under scale code s as 8 values of the type; above top_scale()
+// dequantise_any(). e2m1 has an instruction for it; int8 goes through unsigned bytes, whose
+// conversion is a plain one: (u - 128) 2^e is one fused step, exact.
+template <int FMT, int DT>
+__device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
+  u32x4 o;
+  if constexpr (FMT == DSR_MX_FP4) {
+    const float scale = mx_scale(s);
+#define DSR_DQ(K)                                                                            \
+  if constexpr (DT == DSR_DTYPE_BF16)                                                        \
+    o[K] = __builtin_bit_cast(uint32_t,                                                      \
+                              __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w[0], scale, K));    \
+  else                                                                                       \
+    o[K] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(w[0], scale, K));
+    DSR_DQ(0)
+    DSR_DQ(1)
+    DSR_DQ(2)
+    DSR_DQ(3)
+#undef DSR_DQ
   } else {
+    const float e = __builtin_ldexpf(1.0f, (int)s - 133), bias = -128.0f * e;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const uint32_t u = w[h] ^ 0x80808080u;
+      const float x0 = __builtin_fmaf((float)(u & 255u), e, bias);
+      const float x1 = __builtin_fmaf((float)(u >> 8 & 255u), e, bias);
+      const float x2 = __builtin_fmaf((float)(u >> 16 & 255u), e, bias);
+      const float x3 = __builtin_fmaf((float)(u >> 24), e, bias);
+      o[2 * h] = pack2<DT>(x0, x1);
+      o[2 * h + 1] = pack2<DT>(x2, x3);
+    }
+  }
+  return o;
+}
+
+// The same for any scale code: saturated; NaN under 255.
+template <int FMT, int DT>
+__device__ __forceinline__ u32x4 dequantise_any(const uint32_t* w, uint32_t s) {
+  float x[8];
+  mx_decode<FMT>(uint2{w[0], FMT == DSR_MX_FP4 ? 0u : w[1]}, s, x);
+  constexpr uint32_t top = DT == DSR_DTYPE_BF16 ? 0x7f7f7f7fu : 0x7bff7bffu;
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t p = pack2<DT>(x[2 * k], x[2 * k + 1]), mag = p & 0x7fff7fffu;
+    const u16x2 m = __builtin_elementwise_min(__builtin_bit_cast(u16x2, mag),
+                                              __builtin_bit_cast(u16x2, top));
+    v[k] = s == 255u ? (DT == DSR_DTYPE_BF16 ? 0x7fc07fc0u : 0x7e007e00u)
+                     : (p & 0x80008000u) | __builtin_bit_cast(uint32_t, m);
+  }
+  return v;
+}
+
+// 8 floats as a cache vector; odd: they may be NaN or past the type's largest, where the
+// vector is made with care (saturated, NaN canonical).
+template <int DT>
+__device__ __forceinline__ u32x4 mx_store_vec(float* y, bool odd) {
+  u32x4 v;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) v[k] = pack2<DT>(y[2 * k], y[2 * k + 1]);
+  if (__builtin_expect(odd, 0)) {
+    const float top = DT == DSR_DTYPE_BF16 ? __uint_as_float(0x7f7f0000u) : 65504.0f;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      y[e] = y[e] > top ? top : y[e];
+      y[e] = y[e] < -top ? -top : y[e];
+    }
     v = Codec<DT>::encode(y);
   }
   return v;
@@ -192,43 +269,86 @@ __device__ __forceinline__ MxHalf mx_half(const MxArgs& a, const uint8_t* rec, i
 
 template <int FMT>
 __device__ __forceinline__ uint2 mx_load_codes(const MxHalf& h, int vec) {
-  if (FMT == DSR_MX_FP4) return uint2{reinterpret_cast<const uint32_t*>(h.codes)[vec], 0u};
-  return reinterpret_cast<const uint2*>(h.codes)[vec];
+  if (FMT == DSR_MX_FP4)
+    return uint2{__builtin_nontemporal_load(reinterpret_cast<const uint32_t*>(h.codes) + vec), 0u};
+  typedef unsigned int u32x2 __attribute__((ext_vector_type(2)));
+  const u32x2 w = __builtin_nontemporal_load(reinterpret_cast<const u32x2*>(h.codes) + vec);
+  return uint2{w[0], w[1]};
 }
 
-// Cache vector of record vector `rv`, whose row in the record is that of (t, h), read
-// and, for K, rotated by table `cs` (null: not); c: the vector's column in its row.
+// One vector (8 elements) of a record as loaded; K of a moved page: its neox partner's too.
+struct MxVec {
+  uint2 own, other;
+  uint32_t s, s_other;
+};
+template <int FMT>
+__device__ __forceinline__ MxVec mx_load_vec(const MxHalf& half, int rv, int partner) {
+  MxVec v;
+  v.own = mx_load_codes<FMT>(half, rv);
+  v.s = half.scales[rv >> 2];
+  if (partner >= 0) {
+    v.other = mx_load_codes<FMT>(half, partner);
+    v.s_other = half.scales[partner >> 2];
+  }
+  return v;
+}
+// As a cache vector, not rotated.
+template <int FMT, int DT>
+__device__ __forceinline__ u32x4 mx_plain_vec(const MxVec& v) {
+  const uint32_t w[2] = {v.own.x, v.own.y};
+  u32x4 o = dequantise<FMT, DT>(w, v.s);
+  if (__builtin_expect(v.s > top_scale<FMT, DT>(), 0)) o = dequantise_any<FMT, DT>(w, v.s);
+  return o;
+}
+// Rotated: c is the vector's column in its row, t its pairs' (cos, sin) two by two (neox 4,
+// gptj 2 of them). The sines' products are rounded and the sums fused, as everywhere.
 template <int FMT, int DT, int STYLE>
-__device__ __forceinline__ u32x4 mx_read_vec(const MxHalf& half, int rv, int c, const MxRope& r,
-                                             const float2* cs) {
+__device__ __forceinline__ u32x4 mx_turned_vec(const MxVec& v, int c, const MxRope& r,
+                                               const f32x4* t) {
   float x[8];
-  mx_decode<FMT>(mx_load_codes<FMT>(half, rv), half.scales[rv >> 2], x);
-  if (cs && c < r.rot_vecs) {
-    float t[8];
-    if (STYLE == DSR_ROPE_NEOX) {
-      const bool lower = c < r.half_vecs;
-      const int pv = lower ? rv + r.half_vecs : rv - r.half_vecs;
-      mx_decode<FMT>(mx_load_codes<FMT>(half, pv), half.scales[pv >> 2], t);
-      const float2* p = cs + (lower ? c : c - r.half_vecs) * 8;
+  mx_decode<FMT>(v.own, v.s, x);
+  bool odd = v.s >= top_scale<FMT, DT>();  // sums reach 1.42 times the larger element
+  if (STYLE == DSR_ROPE_NEOX) {
+    float y[8];
+    mx_decode<FMT>(v.other, v.s_other, y);
+    odd |= v.s_other >= top_scale<FMT, DT>();
+    const bool lower = c < r.half_vecs;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 w = p[e];
-        const float ps = t[e] * w.y;
-        x[e] = __builtin_fmaf(x[e], w.x, lower ? -ps : ps);
-      }
-    } else {
-      const float2* p = cs + c * 4;
+    for (int e = 0; e < 8; ++e) {
+      const float ps = y[e] * t[e >> 1][2 * (e & 1) + 1];
+      x[e] = __builtin_fmaf(x[e], t[e >> 1][2 * (e & 1)], lower ? -ps : ps);
+    }
+  } else {
 #pragma unroll
-      for (int e = 0; e < 8; e += 2) {
-        const float2 w = p[e / 2];
-        const float u = x[e], v = x[e + 1];
-        const float us = u * w.y, vs = v * w.y;
-        x[e] = __builtin_fmaf(u, w.x, -vs);
-        x[e + 1] = __builtin_fmaf(v, w.x, us);
-      }
+    for (int e = 0; e < 8; e += 2) {
+      const float cs = t[e >> 2][e & 2], sn = t[e >> 2][(e & 2) + 1];
+      const float u = x[e], w = x[e + 1];
+      const float us = u * sn, ws = w * sn;
+      x[e] = __builtin_fmaf(u, cs, -ws);
+      x[e + 1] = __builtin_fmaf(w, cs, us);
     }
   }
-  return mx_store_vec<DT>(x);
+  return mx_store_vec<DT>(x, odd);
+}
+
+// The record vector that K's vector rv (column c of its row) turns with, or -1.
+template <int STYLE>
+__device__ __forceinline__ int mx_partner(const MxRope& r, int rv, int c) {
+  if (STYLE != DSR_ROPE_NEOX || !r.rope_idx || c >= r.rot_vecs) return -1;
+  return c < r.half_vecs ? rv + r.half_vecs : rv - r.half_vecs;
+}
+// K's vector, loaded with its partner, for table cs (null: not rotated).
+template <int FMT, int DT, int STYLE>
+__device__ __forceinline__ u32x4 mx_key_vec(const MxVec& v, int c, const MxRope& r,
+                                            const float2* cs) {
+  if (!cs || c >= r.rot_vecs) return mx_plain_vec<FMT, DT>(v);
+  constexpr bool kNeox = STYLE == DSR_ROPE_NEOX;
+  const int col = kNeox ? (c < r.half_vecs ? c : c - r.half_vecs) * 8 : c * 4;
+  const f32x4* p = reinterpret_cast<const f32x4*>(cs + col);
+  f32x4 t[4];
+#pragma unroll
+  for (int k = 0; k < (kNeox ? 4 : 2); ++k) t[k] = p[k];
+  return mx_turned_vec<FMT, DT, STYLE>(v, c, r, t);
 }
 
 // Table of entry p in record layer l, or null.
@@ -278,41 +398,63 @@ __device__ __forceinline__ bool mx_pos(const MxArgs& a, const FlatMap& m, const 
   return true;
 }
 
-// Pages -> records. A wave takes 64 vectors of K and of V in the record's order.
-template <int FMT, int DT, bool HND>
+// Pages -> records. A wave takes 64 U vectors of K and of V in the record's order: rows of
+// the cache page (256 bytes at head_dim 128) are read whole, codes and scales of U KiB of
+// the cache go through the wave's LDS and are stored 16 bytes to a lane.
+template <int FMT, int DT, bool HND, int U, int POLICY>
 __global__ __launch_bounds__(kThreads) void kv_mx_gather_kernel(MxArgs a, const int32_t* page_ids,
                                                                 const int64_t* slot_offsets,
                                                                 FlatMap m) {
+  constexpr int CB = mx_code_bytes<FMT>();
+  __shared__ u32x4 lds[kThreads / kWave][(U * kWave * CB + U * 16) / 16];
   MxPos u;
   if (!mx_pos<true>(a, m, page_ids, slot_offsets, &u)) return;
-  const int rv = u.part * kWave + (int)threadIdx.x % kWave;
-  const bool in = rv < a.vecs;
-  int cv = rv;
-  if (!HND) {
-    const int row = (int)div_by((uint32_t)rv, a.row_vecs);
-    const int c = rv - row * (int)a.row_vecs.d;
-    const int h = (int)div_by((uint32_t)row, a.by_block);
-    const int t = row - h * a.block;
-    cv = (t * a.heads + h) * (int)a.row_vecs.d + c;
+  const int lane = (int)threadIdx.x % kWave;
+  const int first = u.part * (kWave * U);
+  const int left = a.vecs - first < kWave * U ? a.vecs - first : kWave * U;
+  uint8_t* const mine = reinterpret_cast<uint8_t*>(lds[threadIdx.x / kWave]);
+  u32x4 x[2][U];
+#pragma unroll
+  for (int k = 0; k < U; ++k) {
+    const int rv = first + k * kWave + lane;
+    int cv = rv;
+    if (!HND) {
+      const int row = (int)div_by((uint32_t)rv, a.row_vecs);
+      const int c = rv - row * (int)a.row_vecs.d;
+      const int h = (int)div_by((uint32_t)row, a.by_block);
+      cv = ((row - h * a.block) * a.heads + h) * (int)a.row_vecs.d + c;
+    }
+    const int off = rv < a.vecs ? cv << 4 : (int)a.page_bytes;
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      x[half][k] = bload(make_rsrc(u.cache + (half ? a.kv_stride : 0), a.page_bytes), off);
   }
 #pragma unroll
   for (int half = 0; half < 2; ++half) {
-    const rsrc_t r = make_rsrc(u.cache + (half ? a.kv_stride : 0), a.page_bytes);
-    const u32x4 v = bload(r, in ? cv << 4 : (int)a.page_bytes);
-    const uint32_t s = mx_scale_code<FMT>(mx_block_max<DT>(v));
-    const uint2 q = mx_encode<FMT, DT>(v, s);
-    if (!in) continue;
+#pragma unroll
+    for (int k = 0; k < U; ++k) {
+      const uint32_t s = mx_scale_code<FMT>(mx_block_max<DT>(x[half][k]));
+      const uint2 q = mx_encode<FMT, DT>(x[half][k], s);
+      const int i = k * kWave + lane;
+      if (FMT == DSR_MX_FP4) reinterpret_cast<uint32_t*>(mine)[i] = q.x;
+      else reinterpret_cast<uint2*>(mine)[i] = q;
+      if ((lane & 3) == 0) mine[U * kWave * CB + (i >> 2)] = (uint8_t)s;
+    }
     const MxHalf o = mx_half(a, u.rec, half);
-    if (FMT == DSR_MX_FP4)
-      reinterpret_cast<uint32_t*>(const_cast<uint8_t*>(o.codes))[rv] = q.x;
-    else
-      reinterpret_cast<uint2*>(const_cast<uint8_t*>(o.codes))[rv] = q;
-    if ((rv & 3) == 0) const_cast<uint8_t*>(o.scales)[rv >> 2] = (uint8_t)s;
+    const rsrc_t codes = make_rsrc(o.codes + (int64_t)first * CB, (int64_t)left * CB);
+    const rsrc_t scales = make_rsrc(o.scales + first / 4, left / 4);
+#pragma unroll
+    for (int k = 0; k < (U * CB + 15) / 16; ++k) {
+      const int i = k * kWave + lane;
+      if (i * 16 < U * kWave * CB) bstore_as<POLICY>(codes, i * 16, reinterpret_cast<u32x4*>(mine)[i]);
+    }
+    if (lane < U * 16)
+      __builtin_amdgcn_raw_buffer_store_b8(mine[U * kWave * CB + lane], scales, lane, 0, POLICY);
   }
 }
 
 // Records -> pages. A wave takes 64 vectors of K and of V in the cache page's order.
-template <int FMT, int DT, bool HND, int STYLE>
+template <int FMT, int DT, bool HND, int STYLE, int POLICY>
 __global__ __launch_bounds__(kThreads) void kv_mx_scatter_kernel(MxArgs a, MxRope r,
                                                                  const int32_t* page_ids,
                                                                  const int64_t* slot_offsets,
@@ -329,11 +471,13 @@ __global__ __launch_bounds__(kThreads) void kv_mx_scatter_kernel(MxArgs a, MxRop
     const int h = row - t * a.heads;
     rv = (h * a.block + t) * (int)a.row_vecs.d + c;
   }
-  const float2* cs = mx_table(r, u.page, u.layer);
-  const u32x4 k = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 0), rv, c, r, cs);
-  const u32x4 v = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 1), rv, c, r, nullptr);
-  *reinterpret_cast<u32x4*>(u.cache + ((int64_t)cv << 4)) = k;
-  *reinterpret_cast<u32x4*>(u.cache + a.kv_stride + ((int64_t)cv << 4)) = v;
+  const rsrc_t ck = make_rsrc(u.cache, a.page_bytes), cw = make_rsrc(u.cache + a.kv_stride, a.page_bytes);
+  // the loads go out before the page's table is known
+  const MxVec v = mx_load_vec<FMT>(mx_half(a, u.rec, 1), rv, -1);
+  const MxVec w = mx_load_vec<FMT>(mx_half(a, u.rec, 0), rv, mx_partner<STYLE>(r, rv, c));
+  const u32x4 k = mx_key_vec<FMT, DT, STYLE>(w, c, r, mx_table(r, u.page, u.layer));
+  bstore_as<POLICY>(ck, cv << 4, k);
+  bstore_as<POLICY>(cw, cv << 4, mx_plain_vec<FMT, DT>(v));
 }
 
 // The token form: lane = one vector of one token's K and V rows, layer blockIdx.y.
@@ -402,8 +546,10 @@ __global__ __launch_bounds__(kThreads) void kv_mx_scatter_slots_kernel(MxArgs a,
   const int l = a.first + (int)blockIdx.y;
   if (!mx_token<HND>(a, slots, rows, n, per_token, l, &u)) return;
   const float2* cs = mx_table(r, u.token, a.layer0 + l);
-  const u32x4 k = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 0), u.rv, u.c, r, cs);
-  const u32x4 v = mx_read_vec<FMT, DT, STYLE>(mx_half(a, u.rec, 1), u.rv, u.c, r, nullptr);
+  const MxVec x = mx_load_vec<FMT>(mx_half(a, u.rec, 1), u.rv, -1);
+  const MxVec w = mx_load_vec<FMT>(mx_half(a, u.rec, 0), u.rv, mx_partner<STYLE>(r, u.rv, u.c));
+  const u32x4 v = mx_plain_vec<FMT, DT>(x);
+  const u32x4 k = mx_key_vec<FMT, DT, STYLE>(w, u.c, r, cs);
   *reinterpret_cast<u32x4*>(u.cache + ((int64_t)u.cv << 4)) = k;
   *reinterpret_cast<u32x4*>(u.cache + a.kv_stride + ((int64_t)u.cv << 4)) = v;
 }

@@ -56,6 +56,7 @@ int mx_rope(const dsr_mx_args* in, const dsr_mx_rope* rope, MxRope* r) {
   if (rope->style != DSR_ROPE_NEOX && rope->style != DSR_ROPE_GPTJ) return DSR_ERR_ARG;
   if (rope->n_tables < 0 || (rope->layer_group && rope->n_groups < 1)) return DSR_ERR_ARG;
   if (!rope->rope_idx || (rope->n_tables > 0 && !rope->cos_sin)) return DSR_ERR_ARG;
+  if (!aligned16p(rope->cos_sin)) return DSR_ERR_ALIGN;
   const int rd = rope->rot_dim;
   if (rd <= 0 || rd > in->head_dim || rd % (rope->style == DSR_ROPE_NEOX ? 16 : 8))
     return DSR_ERR_SHAPE;
@@ -87,16 +88,43 @@ void mx_dispatch(const dsr_mx_args* in, F f) {
 #undef DSR_MX_HND
 }
 
+// Launch shape of the page form, by the bytes of cache it moves. Over 200 MiB (as the copies'
+// copy_shape) the stores are nt sc0 sc1 in chunks of workgroups. Llama-3-8B, 79,906 tokens
+// saved in mxint8 (15.9 GB) and loaded, Llama-3-8B 81,920 loaded rotated (16.3 GB), fp16
+// Qwen2.5-7B head-major from mxfp4 (1.70 GB):
+//   save: 4 pieces a wave, 4 workgroups a CU 2.72 ms (5.83 TB/s); 1 piece 3.77, 2 2.75, 8 2.89,
+//     6 a CU 2.79; stores nt 2.77, sc0 sc1 2.95;
+//   load: 6 a CU 2.68 ms (5.92 TB/s), 4 2.86, 5 2.86, 8 2.74; nt 2.72, sc0 sc1 2.93. From e2m1,
+//     a quarter of whose bytes are reads, and where K turns, a wave's life is latency, not
+//     bytes: 8 a CU 287 us (322 at 6, 366 at 4) and 3.14 ms (3.36 at 6, 4.06 at 4).
+// Below, nt and one piece a wave: the launch is over with its first waves.
+constexpr int64_t kMxLarge = 200 << 20;
+constexpr int kMxPieces = 4, kMxGatherWgPerCu = 4, kMxScatterWgPerCu = 6, kMxTurnWgPerCu = 8;
+struct MxShape {
+  bool large;
+  uint32_t chunk;
+  int pieces;  // vectors of 64 per wave
+};
+MxShape mx_shape(const MxArgs& a, int64_t units) {
+  const bool large = 2 * a.page_bytes * units > kMxLarge;
+  return {large, large ? kChunk : 0u, large ? kMxPieces : 1};
+}
+
 struct GatherPages {
   const MxArgs& a;
   const int32_t* ids;
   const int64_t* offs;
   const FlatMap& m;
   unsigned grid;
+  size_t dyn;
+  bool large;
   hipStream_t s;
   template <int FMT, int DT, bool HND>
   void operator()() const {
-    kv_mx_gather_kernel<FMT, DT, HND><<<grid, kThreads, 0, s>>>(a, ids, offs, m);
+    if (large)
+      kv_mx_gather_kernel<FMT, DT, HND, kMxPieces, kStoreNtSc><<<grid, kThreads, dyn, s>>>(a, ids, offs, m);
+    else
+      kv_mx_gather_kernel<FMT, DT, HND, 1, kStoreNt><<<grid, kThreads, dyn, s>>>(a, ids, offs, m);
   }
 };
 struct ScatterPages {
@@ -107,13 +135,21 @@ struct ScatterPages {
   const int64_t* offs;
   const FlatMap& m;
   unsigned grid;
+  size_t dyn;
+  bool large;
   hipStream_t s;
   template <int FMT, int DT, bool HND>
   void operator()() const {
-    if (style == DSR_ROPE_NEOX)
-      kv_mx_scatter_kernel<FMT, DT, HND, DSR_ROPE_NEOX><<<grid, kThreads, 0, s>>>(a, r, ids, offs, m);
-    else
-      kv_mx_scatter_kernel<FMT, DT, HND, DSR_ROPE_GPTJ><<<grid, kThreads, 0, s>>>(a, r, ids, offs, m);
+#define DSR_MX_SCATTER(STYLE, POLICY) \
+  kv_mx_scatter_kernel<FMT, DT, HND, STYLE, POLICY><<<grid, kThreads, dyn, s>>>(a, r, ids, offs, m)
+    if (style == DSR_ROPE_NEOX) {
+      if (large) DSR_MX_SCATTER(DSR_ROPE_NEOX, kStoreNtSc);
+      else DSR_MX_SCATTER(DSR_ROPE_NEOX, kStoreNt);
+    } else {
+      if (large) DSR_MX_SCATTER(DSR_ROPE_GPTJ, kStoreNtSc);
+      else DSR_MX_SCATTER(DSR_ROPE_GPTJ, kStoreNt);
+    }
+#undef DSR_MX_SCATTER
   }
 };
 struct Tokens {
@@ -183,9 +219,14 @@ int dsr_gather_mx(const dsr_mx_args* args, int first, int count, const int32_t* 
   const int rc = mx_args(args, first, count, page_ids, slot_offsets, n_pages, &a);
   if (rc != DSR_OK || n_pages == 0 || count == 0) return rc;
   if ((int64_t)n_pages * count > 0x7fffffffLL) return DSR_ERR_ARG;
-  return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, count, 0,
+  const MxShape c = mx_shape(a, (int64_t)n_pages * count);
+  const int64_t per = kWave * c.pieces;
+  const int cb = args->format == DSR_MX_FP4 ? 4 : 8;
+  const size_t dyn = occupancy_lds(kMxGatherWgPerCu, (kThreads / kWave) * (per * cb + c.pieces * 16));
+  return launch_flat((int64_t)n_pages * count, (a.vecs + per - 1) / per, count, c.chunk,
                      [&](const FlatMap& m, unsigned grid) {
-    mx_dispatch(args, GatherPages{a, page_ids, slot_offsets, m, grid, (hipStream_t)stream});
+    mx_dispatch(args, GatherPages{a, page_ids, slot_offsets, m, grid, dyn, c.large,
+                                  (hipStream_t)stream});
   });
 }
 
@@ -198,10 +239,12 @@ int dsr_scatter_mx(const dsr_mx_args* args, int first, int count, const int32_t*
   if (rc != DSR_OK || n_pages == 0 || count == 0) return rc;
   if ((rc = mx_rope(args, rope, &r)) != DSR_OK) return rc;
   if ((int64_t)n_pages * count > 0x7fffffffLL) return DSR_ERR_ARG;
-  return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, n_pages, 0,
+  const MxShape c = mx_shape(a, (int64_t)n_pages * count);
+  const size_t dyn = occupancy_lds(rope || args->format == DSR_MX_FP4 ? kMxTurnWgPerCu : kMxScatterWgPerCu, 0);
+  return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, n_pages, c.chunk,
                      [&](const FlatMap& m, unsigned grid) {
     mx_dispatch(args, ScatterPages{a, r, rope ? rope->style : DSR_ROPE_NEOX, page_ids,
-                                   slot_offsets, m, grid, (hipStream_t)stream});
+                                   slot_offsets, m, grid, dyn, c.large, (hipStream_t)stream});
   });
 }
 
