@@ -99,7 +99,8 @@ void mx_dispatch(const dsr_mx_args* in, F f) {
 //     bytes: 8 a CU 287 us (322 at 6, 366 at 4) and 3.14 ms (3.36 at 6, 4.06 at 4).
 // Below, nt and one piece a wave: the launch is over with its first waves.
 constexpr int64_t kMxLarge = 200 << 20;
-constexpr int kMxPieces = 4, kMxGatherWgPerCu = 4, kMxScatterWgPerCu = 6, kMxTurnWgPerCu = 8;
+constexpr int kMxPieces = 4, kMxGatherWgPerCu = 4, kMxScatterWgPerCu = 6, kMxTurnWgPerCu = 8,
+              kMxPairsWgPerCu = 5;
 struct MxShape {
   bool large;
   uint32_t chunk;
@@ -150,6 +151,27 @@ struct ScatterPages {
       else DSR_MX_SCATTER(DSR_ROPE_GPTJ, kStoreNt);
     }
 #undef DSR_MX_SCATTER
+  }
+};
+struct ScatterPairs {
+  const MxArgs& a;
+  const MxRope& r;
+  const int32_t* ids;
+  const int64_t* offs;
+  const FlatMap& m;
+  unsigned grid;
+  size_t dyn;
+  bool large;
+  hipStream_t s;
+  template <int FMT, int DT, bool HND>
+  void operator()() const {
+    const FastDiv half = fast_div((uint32_t)r.half_vecs);
+    if (large)
+      kv_mx_scatter_pairs_kernel<FMT, DT, HND, kStoreNtSc>
+          <<<grid, kThreads, dyn, s>>>(a, r, ids, offs, m, half);
+    else
+      kv_mx_scatter_pairs_kernel<FMT, DT, HND, kStoreNt>
+          <<<grid, kThreads, dyn, s>>>(a, r, ids, offs, m, half);
   }
 };
 struct Tokens {
@@ -240,6 +262,14 @@ int dsr_scatter_mx(const dsr_mx_args* args, int first, int count, const int32_t*
   if ((rc = mx_rope(args, rope, &r)) != DSR_OK) return rc;
   if ((int64_t)n_pages * count > 0x7fffffffLL) return DSR_ERR_ARG;
   const MxShape c = mx_shape(a, (int64_t)n_pages * count);
+  if (rope && rope->style == DSR_ROPE_NEOX && rope->rot_dim == args->head_dim) {
+    const size_t lds = occupancy_lds(kMxPairsWgPerCu, 0);
+    return launch_flat((int64_t)n_pages * count, (a.vecs / 2 + kWave - 1) / kWave, n_pages, c.chunk,
+                       [&](const FlatMap& m, unsigned grid) {
+      mx_dispatch(args, ScatterPairs{a, r, page_ids, slot_offsets, m, grid, lds, c.large,
+                                     (hipStream_t)stream});
+    });
+  }
   const size_t dyn = occupancy_lds(rope || args->format == DSR_MX_FP4 ? kMxTurnWgPerCu : kMxScatterWgPerCu, 0);
   return launch_flat((int64_t)n_pages * count, (a.vecs + kWave - 1) / kWave, n_pages, c.chunk,
                      [&](const FlatMap& m, unsigned grid) {
