@@ -157,6 +157,8 @@ SIGNATURES = {
     "dsr_plan_gather": ([_P, _P, _I, _I64, _I64, _I64, _I64, _P, _I64, _P], _I),
     "dsr_plan_slots": (
         [_P, _P, _P, _I, _I64, _I, _I64, _I64, _I64, _I, _I, _P, _I64, _P], _I),
+    "dsr_plan_slots_mx": (
+        [_P, _P, _P, _I, _I64, _I, _I64, _I64, _I, _I, _P, _I64, _P], _I),
     "dsr_put": ([_P, _P, _I64, _P], _I),
     "dsr_delta_tables": ([_P, _I, _I, _P, _P], _I),
     "dsr_gather_layers": ([_P, _I, _I, _P], _I),

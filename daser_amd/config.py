@@ -25,10 +25,12 @@ class DaserConfig:
     block_tokens: int = 16
     dtype_bytes: int = 2
     model_id: str = "default"
+    record_format: str = ""  # "mxint8" / "mxfp4": quantised records (not in the reference)
 
     def resolved_slot_size(self) -> int:
         """slot_size if set, else num_kv_heads * head_dim * 2 (K and V) *
-        num_layers * block_tokens * dtype_bytes; raises ValueError naming the
+        num_layers * block_tokens * dtype_bytes, or a quantised record's bytes
+        with record_format; raises ValueError naming the
         first missing model parameter (reference :47-75)."""
         if self.slot_size > 0:
             return self.slot_size
@@ -37,5 +39,10 @@ class DaserConfig:
             if value == 0:
                 raise ValueError(f"slot_size is 0 but {name} is also 0; "
                                  "provide either slot_size or all model params")
+        if self.record_format:
+            from daser_amd.mx import MXFormat
+
+            return MXFormat(self.record_format, self.num_layers, self.block_tokens,
+                            self.num_kv_heads, self.head_dim).slot_bytes
         return (self.num_kv_heads * self.head_dim * 2 * self.num_layers * self.block_tokens
                 * self.dtype_bytes)

@@ -349,6 +349,7 @@ class DaserConnector(KVConnectorBase_V1):
                 io_backend=extra.get("io_backend", "mmap"),
                 save_stream=extra.get("save_stream", "auto"),
                 cache_geometry=geometry,
+                record_format=extra.get("record_format"),
             )
             self._k_scale_cfg = extra.get("k_scale")  # uniform fp8 K scale, optional
             self._async_save = bool(extra.get("async_save", False))

@@ -342,4 +342,78 @@ int dsr_plan_slots(const int64_t* slots, const int64_t* rows, const int64_t* rop
   }
 }
 
+int dsr_plan_slots_mx(const int64_t* slots, const int64_t* rows, const int64_t* rope_idx, int n,
+                      int64_t num_blocks, int block_size, int64_t rec_end, int64_t staging_bytes,
+                      int n_tables, int mode, void* out, int64_t out_bytes, dsr_plan* plan) {
+  if (n < 0 || !plan || (n > 0 && (!slots || !rows || !out)) || num_blocks < 0 ||
+      block_size <= 0 || rec_end < 0 || (mode != 0 && mode != 1) ||
+      num_blocks > INT64_MAX / block_size)
+    return DSR_ERR_ARG;
+  memset(plan, 0, sizeof(*plan));
+  if (out_bytes < DSR_PLAN_BYTES(n)) return DSR_ERR_TOO_LARGE;
+  const int64_t num_slots = num_blocks * block_size;
+  const int64_t* const key = mode ? rows : slots;  // what is written
+  // Entries come in runs (the tokens of a page): stretches of consecutive slots and rows,
+  // checked and ordered whole.
+  struct Run {
+    int64_t key;
+    int32_t first, count;
+  };
+  try {
+    std::vector<Run> runs;
+    for (int i = 0; i < n; ++i) {
+      if (rope_idx && (rope_idx[i] < -1 || rope_idx[i] >= n_tables)) return DSR_PLAN_ERR_ROPE;
+      if (slots[i] < 0) continue;
+      if (slots[i] >= num_slots) return DSR_PLAN_ERR_SLOT;
+      if (!runs.empty() && runs.back().first + runs.back().count == i &&
+          slots[i] == slots[i - 1] + 1 && rows[i] == rows[i - 1] + 1)
+        ++runs.back().count;
+      else
+        runs.push_back({key[i], i, 1});
+    }
+    auto before = [](const Run& x, const Run& y) {
+      return x.key != y.key ? x.key < y.key : x.first < y.first;
+    };
+    std::sort(runs.begin(), runs.end(), before);
+    bool twice = false;
+    for (size_t r = 1; r < runs.size(); ++r)
+      twice |= runs[r].key < runs[r - 1].key + runs[r - 1].count;
+    if (twice) {  // entry by entry, of a slot (a save: of a row) the last one
+      std::vector<Run> each;
+      for (const Run& r : runs)
+        for (int i = 0; i < r.count; ++i) each.push_back({r.key + i, r.first + i, 1});
+      std::sort(each.begin(), each.end(), before);
+      runs.clear();
+      for (size_t i = 0; i < each.size(); ++i)
+        if (i + 1 == each.size() || each[i].key != each[i + 1].key) runs.push_back(each[i]);
+    }
+    int m = 0;
+    for (const Run& r : runs) {
+      const int64_t row = rows[r.first], off = row / block_size;
+      if (row < 0 || check_record(off, rec_end, staging_bytes)) return DSR_PLAN_ERR_ROW;
+      // past the record's last row the next name is that of an odd offset
+      if ((off & 15) || row - off * block_size + r.count > block_size) return DSR_PLAN_ERR_ALIGN;
+      m += r.count;
+    }
+    uint8_t* const base = static_cast<uint8_t*>(out);
+    plan->n_pages = m;
+    plan->off_ids = round16(8 * (int64_t)m);
+    plan->off_rope = plan->off_ids + round16(8 * (int64_t)m);
+    plan->bytes = plan->off_rope + (rope_idx ? round16(4 * (int64_t)m) : 0);
+    int64_t* const s = reinterpret_cast<int64_t*>(base);
+    int64_t* const t = reinterpret_cast<int64_t*>(base + plan->off_ids);
+    int32_t* const rope = reinterpret_cast<int32_t*>(base + plan->off_rope);
+    int k = 0;
+    for (const Run& r : runs)
+      for (int i = r.first; i < r.first + r.count; ++i, ++k) {
+        s[k] = slots[i];
+        t[k] = rows[i];
+        if (rope_idx) rope[k] = (int32_t)rope_idx[i];
+      }
+    return DSR_OK;
+  } catch (const std::bad_alloc&) {
+    return DSR_ERR_TOO_LARGE;
+  }
+}
+
 }  // extern "C"

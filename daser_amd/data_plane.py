@@ -178,13 +178,23 @@ class KVDataPlane:
                  k_scales: Optional[torch.Tensor] = None, io_readers: int = 4,
                  layer_rope: Optional[list] = None,
                  io_timeout: Optional[float] = 120.0,
-                 cache_geometry: Optional[dict] = None) -> None:
+                 cache_geometry: Optional[dict] = None,
+                 record_format: Optional[str] = None) -> None:
+        """``record_format``: "mxint8" or "mxfp4" for quantised records
+        (daser_amd.mx), None for records in the caches' own type."""
         if save_mode not in ("per_layer", "deferred"):
             raise ValueError("save_mode must be 'per_layer' or 'deferred'")
         if io_backend not in ("native", "mmap", "direct", "python"):
             raise ValueError("io_backend must be 'native', 'mmap', 'direct' or 'python'")
         if save_stream not in ("side", "current", "auto"):
             raise ValueError("save_stream must be 'side', 'current' or 'auto'")
+        if record_format is not None:
+            from daser_amd.mx import FORMATS
+
+            if record_format not in FORMATS:
+                raise ValueError(f"record_format must be one of {sorted(FORMATS)} or None")
+        self.record_format = record_format
+        self.fmt = None  # mx.MXFormat of the registered caches' records
         self.io_backend = io_backend
         self.save_stream = save_stream
         self._side: Optional[torch.cuda.Stream] = None
@@ -248,6 +258,11 @@ class KVDataPlane:
         self._cache_ptrs = [c.data_ptr() for c in caches]
         lay = self.table.layout
         derived = lay.slot_bytes
+        if self.record_format is not None:
+            from daser_amd import mx
+
+            self.fmt = mx.MXFormat.of(lay, self.record_format)
+            derived = self.fmt.slot_bytes
         if slot_size and slot_size != derived:
             raise ValueError(f"configured slot_size {slot_size} != derived {derived}")
         self.slot_bytes = derived
@@ -310,11 +325,13 @@ class KVDataPlane:
         """Staging arena of a step's store requests. The plan's page tables are
         validated, uploaded and bound to the arena once here; every layer's
         gather reuses them."""
-        from daser_amd import ops
+        from daser_amd import mx, ops
 
         arena = torch.empty(max(plan.arena_bytes, 16), dtype=torch.uint8, device=self.device)
         if plan.page_ids.size:
-            plan.gather = ops.PreparedGather(self.table, plan.page_ids, plan.slot_offsets, arena)
+            plan.gather = ops.PreparedGather(
+                self.table, plan.page_ids, plan.slot_offsets, arena) if self.fmt is None else \
+                mx.PreparedGather(self.table, self.fmt, plan.page_ids, plan.slot_offsets, arena)
             per_layer = plan.page_ids.size * self.table.layout.layer_bytes
             plan.on_side = self._side is not None and (
                 self.save_stream == "side" or per_layer >= SIDE_STREAM_MIN_LAYER_BYTES)
@@ -354,7 +371,7 @@ class KVDataPlane:
         from it (daser_connector.py:627-632), so one that is not the
         registered cache of that layer is gathered from instead (a one-off
         launch through its own table, with a warning)."""
-        from daser_amd import ops
+        from daser_amd import mx, ops
 
         if plan.gather is None:
             return
@@ -372,7 +389,11 @@ class KVDataPlane:
             ids, offs = plan.gather.tables
             stream = self._save_stream(plan)
             with torch.cuda.stream(torch.cuda.ExternalStream(stream, device=self.device)):
-                ops.gather(table, ids, offs, arena, layer0=l)
+                if self.fmt is None:
+                    ops.gather(table, ids, offs, arena, layer0=l)
+                else:
+                    mx.gather(table, mx.MXFormat.of(table.layout, self.record_format), ids, offs,
+                              arena, layer0=l)
             return
         plan.gather(l, 1, self._save_stream(plan))
 
@@ -468,7 +489,7 @@ class KVDataPlane:
         batches of about ``batch_bytes`` (a read larger than that is a batch
         of its own); each batch is scattered as soon as it has landed, so the
         GPU scatters batch i while the reader rings read batch i+1."""
-        from daser_amd import ops, position
+        from daser_amd import mx, ops, position
 
         if plan.page_ids.size == 0:
             return
@@ -516,7 +537,12 @@ class KVDataPlane:
             if sel.size == 0:
                 continue
             src = plan.src_offsets[sel] - base
-            if tabs is None:
+            if self.fmt is not None:
+                how = {} if tabs is None else dict(
+                    cos_sin=tabs, rope_idx=plan.rope_idx[sel], rot_dim=self.rotary_dim,
+                    style=self.rope_style, layer_group=self._layer_group)
+                mx.scatter(self.table, self.fmt, plan.page_ids[sel], src, buf, **how)
+            elif tabs is None:
                 ops.scatter(self.table, plan.page_ids[sel], src, buf,
                             shared_records=plan.shared_records)
             else:

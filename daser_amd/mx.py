@@ -79,7 +79,10 @@ class MXFormat:
 
 
 def _check_format(lay: ops.PagedKVLayout, fmt: MXFormat) -> None:
-    if fmt.num_layers != lay.num_layers or fmt != MXFormat.of(lay, fmt.name):
+    if (fmt.num_layers, fmt.block_size, fmt.num_heads, fmt.head_dim) != \
+            (lay.num_layers, lay.block_size, lay.num_heads, lay.head_dim) or \
+            lay.dtype not in _DTYPES or lay.k_layout == "kx":
+        MXFormat.of(lay, fmt.name)  # says what such caches lack
         raise ValueError(f"{fmt} is not the format of these caches' records")
 
 
@@ -140,13 +143,14 @@ class PreparedGather:
         lay = table.layout
         first, count, nbytes = _prepare(table, fmt, staging, layer0, layers)
         host = _host_pair(page_ids, slot_offsets, _PAGES)
-        plan = None
+        self._plan = self._tables = None
         if host is None:
-            self.tables = _device_pair(lay, page_ids, slot_offsets, torch.int32, torch.int64,
-                                       _PAGES)
+            self._tables = _device_pair(lay, page_ids, slot_offsets, torch.int32, torch.int64,
+                                        _PAGES)
+            self._tail = (self._tables[0].data_ptr(), self._tables[1].data_ptr(),
+                          self._tables[0].numel())
         elif not host[0].size:
-            self.tables = (torch.empty(0, dtype=torch.int32, device=lay.device),
-                           torch.empty(0, dtype=torch.int64, device=lay.device))
+            self._tail = (None, None, 0)
         else:
             ids, offs = host
             lib, span = _lib.lib(), count * fmt.layer_bytes
@@ -157,17 +161,25 @@ class PreparedGather:
                     span + (layer0 + first) * fmt.layer_bytes, span, nbytes, out, size, at),
                     lay.num_blocks)
 
-            plan = ops._HostPlan(ids.size, lay.device, fill)
-            self.tables = (plan.table(plan.plan.off_ids, ids.size, torch.int32),
-                           plan.table(0, ids.size, torch.int64))
-        self._keep = (table, staging, plan)
+            self._plan = plan = ops._HostPlan(ids.size, lay.device, fill)
+            self._tail = (plan.ids, plan.offsets, ids.size)
+        self._keep = (table, staging)
         self._args = _args(table, fmt, staging, nbytes, layer0)
-        self._tail = (self.tables[0].data_ptr(), self.tables[1].data_ptr(),
-                      self.tables[0].numel())
         self._args_ptr = ctypes.addressof(self._args)
         self._range = (first, first + count)
         self._device = lay.device
         self._fn = _lib.lib().dsr_gather_mx
+
+    @property
+    def tables(self) -> tuple[torch.Tensor, torch.Tensor]:
+        """(page_ids, slot_offsets) as device tensors."""
+        if self._tables is None:
+            n, dev = self._tail[2], self._device
+            self._tables = (torch.empty(0, dtype=torch.int32, device=dev),
+                            torch.empty(0, dtype=torch.int64, device=dev)) if not n else (
+                self._plan.table(self._plan.plan.off_ids, n, torch.int32),
+                self._plan.table(0, n, torch.int64))
+        return self._tables
 
     def __call__(self, first: int, count: int, stream: int) -> None:
         """Saves table layers [first, first + count) on ``stream`` (a HIP stream handle)."""
@@ -276,8 +288,10 @@ def _requests(req_tokens, fmt: MXFormat, base: int):
 
 def _slot_tables(lay, fmt: MXFormat, slot_mapping, record_rows, rope_idx, n_tables: int,
                  nbytes: int, last: int, written: bool):
-    """Checked device tables of a token-form call; of a record row (``written``) or cache
-    slot listed more than once the last entry stays, as sequential copies would leave it."""
+    """Addresses of a token-form call's device tables (slots, rows, rope) with the number of
+    tokens, and what holds them. Host tables are planned by the library: of a record row
+    (``written``) or cache slot listed more than once the last entry stays, as sequential
+    copies would leave it."""
     host = _host_pair(slot_mapping, record_rows, _SLOTS)
     ridx = None if rope_idx is None else ops._host_list(rope_idx)
     if host is None or (rope_idx is not None and ridx is None):
@@ -286,33 +300,22 @@ def _slot_tables(lay, fmt: MXFormat, slot_mapping, record_rows, rope_idx, n_tabl
             tables.append(ops._as_device_table(rope_idx, torch.int32, lay.device, "rope_idx"))
         if any(t.numel() != tables[0].numel() for t in tables):
             raise ValueError("rope_idx and slot_mapping differ in length")
-        return tables
+        at = [t.data_ptr() for t in tables] + [None]
+        return (at[0], at[1], at[2], tables[0].numel()), tables
     slots, rows = host
     if ridx is not None and ridx.size != slots.size:
         raise ValueError("rope_idx and slot_mapping differ in length")
-    keep = np.nonzero(slots >= 0)[0]
-    key = (rows if written else slots)[keep]
-    # in slot order (near-sequential writes); equal keys keep list order: the last stays
-    order = np.argsort(key, kind="stable")
-    key = key[order]
-    if key.size > 1 and (key[1:] == key[:-1]).any():
-        order = order[np.append(key[1:] != key[:-1], True)]
-    keep = keep[order]
-    s, r = slots[keep], rows[keep]
-    if s.size:
-        if s.max() >= lay.num_blocks * lay.block_size:
-            raise IndexError("slot outside the block pool")
-        off = r // fmt.block_size
-        if r.min() < 0 or off.max() + last > nbytes:
-            raise IndexError("token row outside the staging buffer")
-        if (off % 16).any():
-            raise ValueError("slot offsets must be multiples of 16 bytes")
-    both = torch.from_numpy(np.concatenate([s, r]))
-    both = ops._upload(both, lay.device)
-    tables = [both[:s.size], both[s.size:]]
-    if ridx is not None:
-        tables.append(ops._as_device_table(ridx[keep], torch.int32, lay.device, "rope_idx"))
-    return tables
+    if not slots.size:
+        return (None, None, None, 0), None
+    lib = _lib.lib()
+
+    def fill(out: int, size: int, at: int) -> None:
+        ops._plan_check("dsr_plan_slots_mx", lib.dsr_plan_slots_mx(
+            ops._addr(slots), ops._addr(rows), ops._addr(ridx), slots.size, lay.num_blocks,
+            lay.block_size, last, nbytes, n_tables, int(written), out, size, at), lay.num_blocks)
+
+    plan = ops._HostPlan(slots.size, lay.device, fill)
+    return (plan.offsets, plan.ids, plan.rope, plan.plan.n_pages), plan
 
 
 def gather_slots(table: ops.LayerTable, fmt: MXFormat, slot_mapping, record_rows,
@@ -323,13 +326,14 @@ def gather_slots(table: ops.LayerTable, fmt: MXFormat, slot_mapping, record_rows
     other rows stay as they are."""
     lay = table.layout
     first, count, nbytes = _prepare(table, fmt, staging, layer0, layers)
-    tables = _slot_tables(lay, fmt, slot_mapping, record_rows, None, 0, nbytes,
-                          (layer0 + first + count) * fmt.layer_bytes, True)
+    (slots, rows, _, n), _keep = _slot_tables(
+        lay, fmt, slot_mapping, record_rows, None, 0, nbytes,
+        (layer0 + first + count) * fmt.layer_bytes, True)
     args = _args(table, fmt, staging, nbytes, layer0)
     with _current(lay.device):
         _lib.check("dsr_gather_slots_mx", _lib.lib().dsr_gather_slots_mx(
-            ctypes.addressof(args), first, count, tables[0].data_ptr(), tables[1].data_ptr(),
-            tables[0].numel(), ops._stream_handle(lay.device)))
+            ctypes.addressof(args), first, count, slots, rows, n,
+            ops._stream_handle(lay.device)))
 
 
 def scatter_slots(table: ops.LayerTable, fmt: MXFormat, slot_mapping, record_rows,
@@ -342,20 +346,24 @@ def scatter_slots(table: ops.LayerTable, fmt: MXFormat, slot_mapping, record_row
     first, count, nbytes = _prepare(table, fmt, staging, layer0, layers)
     rope = _rope(lay, cos_sin, rope_idx, rot_dim, style, layer0, layer_group)
     r = None if rope is None else rope[0]
-    tables = _slot_tables(lay, fmt, slot_mapping, record_rows, rope_idx,
-                          0 if r is None else r.n_tables, nbytes,
-                          (layer0 + first + count) * fmt.layer_bytes, False)
+    (slots, rows, ridx, n), _keep = _slot_tables(
+        lay, fmt, slot_mapping, record_rows, rope_idx, 0 if r is None else r.n_tables, nbytes,
+        (layer0 + first + count) * fmt.layer_bytes, False)
+    if not n:
+        return
     if r is not None:
-        r.rope_idx = tables[2].data_ptr()
+        r.rope_idx = ridx
     args = _args(table, fmt, staging, nbytes, layer0)
     with _current(lay.device):
         _lib.check("dsr_scatter_slots_mx", _lib.lib().dsr_scatter_slots_mx(
-            ctypes.addressof(args), first, count, tables[0].data_ptr(), tables[1].data_ptr(),
-            tables[0].numel(), None if r is None else ctypes.addressof(r),
+            ctypes.addressof(args), first, count, slots, rows, n, None if r is None else ctypes.addressof(r),
             ops._stream_handle(lay.device)))
 
 
 def _vector(x, dtype: torch.dtype, device: torch.device, name: str, size: Optional[int] = None):
+    if isinstance(x, torch.Tensor) and x.dtype == dtype and x.device == device and \
+            x.dim() == 1 and x.is_contiguous() and (size is None or x.shape[0] == size):
+        return x
     if ops._on_device(x) and x.device != device:
         raise ValueError(f"{name} must live on q's device")
     t = ops._as_device_table(x, dtype, device, name)
@@ -364,7 +372,7 @@ def _vector(x, dtype: torch.dtype, device: torch.device, name: str, size: Option
     return t
 
 
-def _check_host_tables(fmt, q, staging, q_start, page_start, slot_offsets, context, limits, last):
+def _check_host_tables(fmt, q, staging, q_start, page_start, slot_offsets, context, last):
     """Errors of the attention's tables, as far as they are on the host."""
     def starts(x, n, name):
         a = ops._host_list(x)
@@ -430,8 +438,9 @@ def attend(q: torch.Tensor, fmt: MXFormat, staging: torch.Tensor, q_start, page_
     if not 0 <= layer < fmt.num_layers:
         raise IndexError("layer outside the records")
     dev = q.device
-    _check_host_tables(fmt, q, staging, q_start, page_start, slot_offsets, context, limits,
-                       (layer + 1) * fmt.layer_bytes)
+    tables = (q_start, page_start, slot_offsets, context)
+    if not all(isinstance(x, torch.Tensor) and x.is_cuda for x in tables):
+        _check_host_tables(fmt, q, staging, *tables, (layer + 1) * fmt.layer_bytes)
     if not q.is_cuda:
         raise ValueError("q must live on a GPU")
     if max_queries is None:

@@ -546,6 +546,17 @@ int dsr_plan_slots(const int64_t* slots, const int64_t* rows, const int64_t* rop
                    int64_t staging_bytes, int n_tables, int mode, void* out, int64_t out_bytes,
                    dsr_slot_plan* plan);
 
+/* The same for the quantised token form (dsr_*_slots_mx): n tokens' slots (negative:
+ * padding) and record rows (record offset * block_size + row). rec_end: bytes from a
+ * record's offset to the end of the last layer that the call moves. mode 0: a load, in
+ * slot order, of a slot listed more than once the last one; mode 1: a save, in the
+ * records' order, of a row listed more than once the last one; the entries left out are
+ * not checked. plan->n_pages tokens: slots (int64) at 0, rows (int64) at off_ids, table
+ * indices (int32) at off_rope. out_bytes: DSR_PLAN_BYTES(n). */
+int dsr_plan_slots_mx(const int64_t* slots, const int64_t* rows, const int64_t* rope_idx, int n,
+                      int64_t num_blocks, int block_size, int64_t rec_end, int64_t staging_bytes,
+                      int n_tables, int mode, void* out, int64_t out_bytes, dsr_plan* plan);
+
 /* Writes up to DSR_PUT_BYTES bytes (a multiple of 4) of host memory to device
  * memory (4-byte aligned) as a kernel's arguments, in stream order: the source
  * may be reused at once. For small tables; a copy costs twice the host time. */
