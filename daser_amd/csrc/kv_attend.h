@@ -305,6 +305,7 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
   const int h = (int)blockIdx.y * g.wave_heads + wave % g.wave_heads;
   const int share = kAttendWaves / g.wave_heads;  // waves of a head
   const int split = (int)blockIdx.x % g.splits, tile0 = (int)blockIdx.x / g.splits;
+  if (tile0 >= g.tiles) return;  // the odd one of the grid
   const AttendRequest rq = attend_request(a, (int)blockIdx.z);
   const int64_t rows = rq.q1 > rq.q0 ? (int64_t)(rq.q1 - rq.q0) * g.group : 0;
   const float ninf = -__builtin_inff();

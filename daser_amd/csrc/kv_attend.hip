@@ -115,7 +115,14 @@ void launch_attend_dims(const AttendArgs& g, dim3 grid, hipStream_t s) {
   }
 }
 void launch_attend(const AttendArgs& g, int n_req, hipStream_t s) {
-  const dim3 grid((unsigned)(g.tiles * g.splits), (unsigned)(g.a.kv_heads / g.wave_heads), (unsigned)n_req);
+  // An odd number of workgroups to a (request, heads): the XCDs are dealt workgroups in
+  // turn, and with an even number the first splits, which every request has, fall to some
+  // of them and the last, which few have, to others (decode batch 174 -> 137 us). Several
+  // tiles of rows are cut to fill the chip once: one more would start a second round
+  // (questions 72 -> 98 us).
+  unsigned x = (unsigned)(g.tiles * g.splits);
+  if (attend_nq(g) == 1) x |= 1u;
+  const dim3 grid(x, (unsigned)(g.a.kv_heads / g.wave_heads), (unsigned)n_req);
   const bool bf16 = g.a.dtype == DSR_DTYPE_BF16;
   if (g.a.format == DSR_MX_FP4) {
     if (bf16) launch_attend_dims<DSR_MX_FP4, DSR_DTYPE_BF16>(g, grid, s);
