@@ -48,6 +48,7 @@ int attend_args(const dsr_attend_args* args, AttendArgs* g, bool* work) {
       return DSR_ERR_SHAPE;
   }
   if (a.n_req == 0 || a.n_q == 0) return DSR_OK;
+  if ((int64_t)a.n_q * a.q_heads > 0x7fffffffLL) return DSR_ERR_ARG;  // rows are 32-bit numbers
   *work = true;
   *g = AttendArgs{};
   g->a = a;

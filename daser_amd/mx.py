@@ -111,7 +111,7 @@ def _prepare(table: ops.LayerTable, fmt: MXFormat, staging: torch.Tensor, layer0
 
 
 def _device_pair(lay, a, b, dtype_a, dtype_b, names):
-    """Tables of a call of which at least one is on the device."""
+    """Checked device tables of a call."""
     a = ops._as_device_table(a, dtype_a, lay.device, names[0])
     b = ops._as_device_table(b, dtype_b, lay.device, names[1])
     if a.numel() != b.numel():
@@ -120,13 +120,31 @@ def _device_pair(lay, a, b, dtype_a, dtype_b, names):
 
 
 def _host_pair(a, b, names):
-    """Both tables as host vectors, or None if one is on the device."""
-    if ops._on_device(a) or ops._on_device(b):
+    """Both tables as host vectors, or None if they are on the device."""
+    on = ops._on_device(a)
+    if on != ops._on_device(b):
+        raise ValueError(f"{names[0]} and {names[1]} must both be host data or device tensors")
+    if on:
         return None
     a, b = ops._host_list(a), ops._host_list(b)
     if a is None or b is None or a.size != b.size:
         raise ValueError(f"{names[0]} and {names[1]} must be vectors of one length")
     return a, b
+
+
+def _host_rope(host, rope_idx, name: str) -> Optional[np.ndarray]:
+    """rope_idx as a host vector where the other tables are; checked device tables are
+    made of it elsewhere."""
+    if rope_idx is None:
+        return None
+    if (host is None) != ops._on_device(rope_idx):
+        raise ValueError(f"rope_idx and {name} must both be host data or device tensors")
+    if host is None:
+        return None
+    ridx = ops._host_list(rope_idx)
+    if ridx is None or ridx.size != host[0].size:
+        raise ValueError(f"rope_idx and {name} differ in length")
+    return ridx
 
 
 _PAGES = ("page_ids", "slot_offsets")
@@ -233,14 +251,8 @@ def scatter(table: ops.LayerTable, fmt: MXFormat, page_ids, slot_offsets, stagin
     lay = table.layout
     first, count, nbytes = _prepare(table, fmt, staging, layer0, layers)
     host = _host_pair(page_ids, slot_offsets, _PAGES)
-    ridx = None if host is None or rope_idx is None else ops._host_list(rope_idx)
-    if host is not None and rope_idx is not None and ridx is None:
-        host = None  # rope_idx on the device
-    n = ops._host_array(page_ids, np.int64).size if host is None and not ops._on_device(
-        page_ids) else (page_ids.numel() if host is None else host[0].size)
-    if rope_idx is not None and (rope_idx.numel() if ops._on_device(rope_idx)
-                                 else np.size(rope_idx)) != n:
-        raise ValueError("rope_idx and page_ids differ in length")
+    ridx = _host_rope(host, rope_idx, "page_ids")
+    n = page_ids.numel() if host is None else host[0].size
     rope = _rope(lay, cos_sin, rope_idx, rot_dim, style, layer0, layer_group)
     if not n:
         return
@@ -263,6 +275,8 @@ def scatter(table: ops.LayerTable, fmt: MXFormat, page_ids, slot_offsets, stagin
         tables = (keep[0].data_ptr(), keep[1].data_ptr(), n)
         if r is not None:
             keep.append(ops._as_device_table(rope_idx, torch.int32, lay.device, "rope_idx"))
+            if keep[2].numel() != n:
+                raise ValueError("rope_idx and page_ids differ in length")
             r.rope_idx = keep[2].data_ptr()
     args = _args(table, fmt, staging, nbytes, layer0)
     with _current(lay.device):
@@ -293,8 +307,8 @@ def _slot_tables(lay, fmt: MXFormat, slot_mapping, record_rows, rope_idx, n_tabl
     (``written``) or cache slot listed more than once the last entry stays, as sequential
     copies would leave it."""
     host = _host_pair(slot_mapping, record_rows, _SLOTS)
-    ridx = None if rope_idx is None else ops._host_list(rope_idx)
-    if host is None or (rope_idx is not None and ridx is None):
+    ridx = _host_rope(host, rope_idx, "slot_mapping")
+    if host is None:
         tables = [*_device_pair(lay, slot_mapping, record_rows, torch.int64, torch.int64, _SLOTS)]
         if rope_idx is not None:
             tables.append(ops._as_device_table(rope_idx, torch.int32, lay.device, "rope_idx"))
@@ -303,8 +317,6 @@ def _slot_tables(lay, fmt: MXFormat, slot_mapping, record_rows, rope_idx, n_tabl
         at = [t.data_ptr() for t in tables] + [None]
         return (at[0], at[1], at[2], tables[0].numel()), tables
     slots, rows = host
-    if ridx is not None and ridx.size != slots.size:
-        raise ValueError("rope_idx and slot_mapping differ in length")
     if not slots.size:
         return (None, None, None, 0), None
     lib = _lib.lib()
@@ -420,8 +432,9 @@ def attend(q: torch.Tensor, fmt: MXFormat, staging: torch.Tensor, q_start, page_
 
     Tables may be host data, checked here, or device tensors, used as they are.
     ``max_queries`` / ``max_context`` are the largest request's, for the launch's
-    shape; None: from host tables, or bounds that hold for any. They do not
-    change results."""
+    shape; None: from host tables, or bounds that hold for any. Results are right
+    whatever they say; how the tokens are split, and so the last bit of a sum, follows
+    them. Rows of ``out`` that belong to no request are left as they were."""
     if q.dim() != 3 or q.dtype not in _DTYPES:
         raise ValueError("q must be bfloat16 or float16 [n, q_heads, head_dim]")
     n, heads, dim = q.shape

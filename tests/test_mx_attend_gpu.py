@@ -180,6 +180,40 @@ def test_long_context_and_wide_split(gpu):
          limits=True).run_and_check()
 
 
+@pytest.mark.parametrize("heads,requests,kw", [
+    (4, 8, dict()), (4, 8, dict(moved=True, limits=True)), (8, 4, dict(name="mxint8", dt="fp16")),
+    (2, 16, dict()), (6, 6, dict(limits=True)), (3, 11, dict(moved=True, style="gptj"))])
+def test_large_launches(gpu, heads, requests, kw):
+    """Where requests, heads and the longest context make a large launch, each wave takes a
+    head of its own (4 or 2 to a workgroup), short and empty requests beside the long one."""
+    contexts = [8200] + [(7 * i * i) % 90 for i in range(requests - 1)]
+    assert requests * heads * 8200 >= 1 << 18
+    Case(gpu, heads=heads, group=2, dim=64, contexts=contexts, queries=[1, 3] * (requests // 2) +
+         [2] * (requests % 2), seed=heads, **kw).run_and_check()
+
+
+def test_many_short_requests(gpu):
+    """A large launch that is not split: the waves write the results themselves."""
+    contexts = [1 + (5 * i) % 32 for i in range(2060)]
+    contexts[7] = 0
+    c = Case(gpu, heads=4, group=1, dim=32, contexts=contexts, queries=[1] * 2060, seed=1)
+    out, lse = c.run_and_check()
+    prior = (torch.randn_like(out), torch.randn_like(lse))
+    both, both_lse = mx.attend(**c.args(), prior=prior)
+    share = torch.sigmoid(prior[1].double() - lse.double())[..., None]
+    o, l, mag, width = c.want()
+    own = torch.from_numpy(o).to(gpu)
+    want = own * (1 - share) + prior[0].double() * share
+    want_lse = torch.logaddexp(torch.from_numpy(l).to(gpu), prior[1].double())
+    # the share is off by what the lse is (some 2^-18), the result by half a step more
+    far = (both.double() - want).abs()
+    half = ref.HALF_STEP["bf16"]
+    tol = torch.from_numpy(mag).to(gpu) * (half * 1.05 + 2.0 ** -16) + half * want.abs() + \
+        2.0 ** -16 * (own.abs() + prior[0].double().abs())
+    assert (far <= tol).all()
+    assert ((both_lse.double() - want_lse).abs() <= 2.0 ** -16 * (1 + want_lse.abs())).all()
+
+
 def test_loud_scores(gpu):
     """Scores of hundreds: the running maximum carries the sum."""
     Case(gpu, contexts=(500, 64), queries=(3, 1), loud=60.0, seed=9).run_and_check()

@@ -439,3 +439,42 @@ def test_on_another_stream(gpu):
         mx.gather(table, fmt, [1, 2], [0, fmt.slot_bytes], rec)
     side.synchronize()
     assert np.array_equal(rec[:fmt.layer_bytes].cpu().numpy(), want_layer(fmt, src[0], 1))
+
+
+@pytest.mark.parametrize("name,dt,layout,bs,heads,dim,pages", [
+    ("mxint8", "bf16", "nhd", 16, 8, 128, 1700), ("mxfp4", "fp16", "hnd", 16, 8, 128, 1700),
+    ("mxfp4", "bf16", "nhd", 5, 3, 96, 19000)])
+def test_large_launches_match_small_ones(gpu, name, dt, layout, bs, heads, dim, pages):
+    """Launches over 200 MiB (other pieces, stores and orders) against the same work in
+    slices of a layer and some pages, which the tests above hold to the definition."""
+    g = torch.Generator(gpu).manual_seed(3)
+    shape = (2, pages, heads, bs, dim) if layout == "hnd" else (2, pages, bs, heads, dim)
+    src = [torch.randn(shape, generator=g, device=gpu).to(ref.TORCH[dt]) for _ in range(2)]
+    view = (lambda x: x.transpose(2, 3)) if layout == "hnd" else (lambda x: x)
+    table = ops.LayerTable([view(x) for x in src])
+    fmt = mx.MXFormat.of(table.layout, name)
+    assert 2 * table.layout.page_bytes * 2 * pages > 200 << 20
+    rng = np.random.default_rng(1)
+    ids, offs = rng.permutation(pages), rng.permutation(pages) * fmt.slot_bytes
+    rec, part = (torch.zeros(pages * fmt.slot_bytes, dtype=torch.uint8, device=gpu)
+                 for _ in range(2))
+    mx.gather(table, fmt, ids, offs, rec)
+    cuts = [(l, slice(i, i + pages // 4 + 1)) for l in (0, 1)
+            for i in range(0, pages, pages // 4 + 1)]
+    for l, s in cuts:
+        mx.gather(table, fmt, ids[s], offs[s], part, layers=(l, 1))
+    assert torch.equal(rec, part)
+    for rot, style in ((0, "neox"), (dim, "neox"), (dim // 2 // 16 * 16, "neox"), (dim, "gptj")):
+        rope, ridx = {}, np.zeros(pages, np.int64)
+        if rot:
+            rope = dict(cos_sin=position.delta_tables([977, -5], rot, THETA, device=gpu),
+                        rot_dim=rot, style=style)
+            ridx = rng.integers(-1, 2, pages)
+        res = [[torch.zeros_like(x) for x in src] for _ in range(2)]
+        to = [ops.LayerTable([view(x) for x in r]) for r in res]
+        mx.scatter(to[0], fmt, ids, offs, rec, **rope, **(dict(rope_idx=ridx) if rot else {}))
+        for l, s in cuts:
+            mx.scatter(to[1], fmt, ids[s], offs[s], rec, layers=(l, 1), **rope,
+                       **(dict(rope_idx=ridx[s]) if rot else {}))
+        for a, b in zip(*res):
+            assert torch.equal(a.view(torch.int16), b.view(torch.int16)), (rot, style)

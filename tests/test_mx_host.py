@@ -138,6 +138,30 @@ def test_token_form_refusals(fn):
         fn(table, fmt, [0, 1], [0], rec)
 
 
+class OnDevice(torch.Tensor):
+    """A tensor that says it is not in host memory."""
+
+    is_cpu = False
+
+
+def test_tables_are_of_one_kind():
+    """Host tables are checked and ordered, device tables used as they are: not both in
+    one call."""
+    table = ops.LayerTable(caches())
+    fmt = mx.MXFormat.of(table.layout, "mxint8")
+    rec = torch.zeros(fmt.slot_bytes, dtype=torch.uint8)
+    there = torch.zeros(1, dtype=torch.int64).as_subclass(OnDevice)
+    for fn in (mx.gather, mx.scatter, mx.gather_slots, mx.scatter_slots):
+        with pytest.raises(ValueError, match="both be host data"):
+            fn(table, fmt, [0], there, rec)
+        with pytest.raises(ValueError, match="both be host data"):
+            fn(table, fmt, there, [0], rec)
+    cs = torch.zeros(1, 32, 2)
+    for fn in (mx.scatter, mx.scatter_slots):
+        with pytest.raises(ValueError, match="both be host data"):
+            fn(table, fmt, [0], [0], rec, cs, there.int())
+
+
 def attend_args(**kw):
     fmt = mx.MXFormat("mxfp4", 2, 16, 2, 64)
     a = dict(q=torch.zeros(3, 4, 64, dtype=torch.bfloat16), fmt=fmt,
