@@ -681,7 +681,7 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
 
 // The splits of a row joined, in their order: a wave to a row, lane s weighing split s,
 // then each lane summing columns.
-template <int DT>
+template <int DT, int D>
 __global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs g) {
   const dsr_attend_args& a = g.a;
   const AttendRequest rq = attend_request(a, (int)blockIdx.z);
@@ -697,13 +697,27 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs 
     int n = seen <= 0 ? 0 : (int)((seen + g.chunk - 1) / g.chunk);
     if (n > g.splits) n = g.splits;
     const float2* ml = g.part_ml + at * g.splits;
-    const float* po = g.part_o + at * g.splits * a.head_dim;
-    float m = ninf;
+    const float* po = g.part_o + at * g.splits * D;
+    // lane s weighs split s; kSum lanes to a row of columns, the others' rows are further
+    // splits. The sums' loads go out before the weights are known.
+    constexpr int kSum = D <= 64 ? 16 : D <= 128 ? 32 : 64, kRows = kWave / kSum, kFar = 8;
+    const int sub = lane / kSum, col = lane % kSum * 4;
+    const bool has = col < D;
+    f32x4 o[kFar];
+    auto fetch = [&](int s0) {
+#pragma unroll
+      for (int k = 0; k < kFar; ++k) {
+        if (s0 + k * kRows >= n) break;
+        const int s = s0 + k * kRows + sub;
+        o[k] = *reinterpret_cast<const f32x4*>(po + (int64_t)(s < n ? s : 0) * D + (has ? col : 0));
+      }
+    };
+    float m = ninf, l = 0.0f;
+    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (n > 0) fetch(0);
     for (int s = lane; s < n; s += kWave) m = __builtin_fmaxf(m, ml[s].x);
 #pragma unroll
     for (int k = 1; k < kWave; k <<= 1) m = __builtin_fmaxf(m, __shfl_xor(m, k));
-    float l = 0.0f;
-    f32x4 sum = {0.0f, 0.0f, 0.0f, 0.0f};
     for (int s0 = 0; s0 < n; s0 += kWave) {
       float w = 0.0f;
       if (s0 + lane < n) {
@@ -713,21 +727,26 @@ __global__ __launch_bounds__(kThreads) void kv_mx_attend_join_kernel(AttendArgs 
           l += x.y * w;
         }
       }
-      const int stop = n - s0 < kWave ? n - s0 : kWave;
-      if (lane * 4 < a.head_dim) {
-#pragma unroll 8
-        for (int s = 0; s < stop; ++s) {
-          const float ws = __uint_as_float(__builtin_amdgcn_readlane((int)__float_as_uint(w), s));
-          const f32x4 o = *reinterpret_cast<const f32x4*>(po + (int64_t)(s0 + s) * a.head_dim + lane * 4);
-          sum += o * ws;
+      for (int s = s0; s < s0 + kWave && s < n; s += kFar * kRows) {
+#pragma unroll
+        for (int k = 0; k < kFar; ++k) {
+          if (s + k * kRows >= n) break;
+          const int at_s = s + k * kRows + sub;
+          const float ws = __shfl(w, (at_s - s0) & (kWave - 1));
+          if (at_s < n) sum += o[k] * ws;
         }
+        if (s + kFar * kRows < n) fetch(s + kFar * kRows);
       }
     }
 #pragma unroll
     for (int k = 1; k < kWave; k <<= 1) l += __shfl_xor(l, k);
+#pragma unroll
+    for (int k = kSum; k < kWave; k <<= 1)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) sum[e] += __shfl_xor(sum[e], k);
     const AttendScale sc = attend_scale(a, at, m, l);
     if (lane == 0) a.lse[at] = sc.lse;
-    if (lane * 4 < a.head_dim) attend_store<DT>(a, at, lane * 4, sum, sc);
+    if (lane < kSum && has) attend_store<DT>(a, at, col, sum, sc);
   }
 }
 

@@ -140,10 +140,18 @@ void launch_attend_join(const AttendArgs& g, int n_req, hipStream_t s) {
   int64_t x = g.a.max_queries < 1 ? 1 : g.a.max_queries;
   if (x > room) x = room < 1 ? 1 : room;
   const dim3 grid((unsigned)x, (unsigned)y, (unsigned)n_req);
-  if (g.a.dtype == DSR_DTYPE_BF16)
-    kv_mx_attend_join_kernel<DSR_DTYPE_BF16><<<grid, kThreads, 0, s>>>(g);
-  else
-    kv_mx_attend_join_kernel<DSR_DTYPE_FP16><<<grid, kThreads, 0, s>>>(g);
+  const bool bf16 = g.a.dtype == DSR_DTYPE_BF16;
+#define DSR_JOIN(D)                                                                       \
+  if (bf16) kv_mx_attend_join_kernel<DSR_DTYPE_BF16, D><<<grid, kThreads, 0, s>>>(g);      \
+  else kv_mx_attend_join_kernel<DSR_DTYPE_FP16, D><<<grid, kThreads, 0, s>>>(g)
+  switch (g.a.head_dim) {
+    case 32: DSR_JOIN(32); break;
+    case 64: DSR_JOIN(64); break;
+    case 96: DSR_JOIN(96); break;
+    case 128: DSR_JOIN(128); break;
+    default: DSR_JOIN(256);
+  }
+#undef DSR_JOIN
 }
 
 }  // namespace

@@ -136,6 +136,16 @@ __device__ __forceinline__ uint2 mx_encode(u32x4 v, uint32_t s) {
   return o;
 }
 
+// Bytes 2 h and 2 h + 1 of w, as int8, times p. A byte u = q + 128 behind 0x64 is the fp16
+// number 1,024 + u, and a fused step takes fp16 in: q p = (1,024 + u) p - 1,152 p, exact. One
+// permutation and two steps for two elements; a conversion for each was one more.
+__device__ __forceinline__ f32x2 int8_pair(uint32_t w, int h, float p, float bias) {
+  const uint32_t v = __builtin_amdgcn_perm(0x64646464u, w ^ 0x80808080u,
+                                           h ? 0x04030402u : 0x04010400u);
+  const f16x2 f = __builtin_bit_cast(f16x2, v);
+  return {__builtin_fmaf((float)f.x, p, bias), __builtin_fmaf((float)f.y, p, bias)};
+}
+
 // Values of 8 codes under scale code s, NaN under 255.
 template <int FMT>
 __device__ __forceinline__ void mx_decode(uint2 c, uint32_t s, float* x) {
@@ -152,14 +162,15 @@ __device__ __forceinline__ void mx_decode(uint2 c, uint32_t s, float* x) {
       x[2 * k + 1] = f[k].y;
     }
   } else {
-    const float p = __builtin_ldexpf(1.0f, (int)s - 133), bias = -128.0f * p;
+    const float p = __builtin_ldexpf(1.0f, (int)s - 133), bias = -1152.0f * p;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const uint32_t u = (e < 4 ? c.x : c.y) ^ 0x80808080u;
-      x[e] = __builtin_fmaf((float)(u >> (8 * (e & 3)) & 255u), p, bias);
+    for (int k = 0; k < 4; ++k) {
+      const f32x2 f = int8_pair(k < 2 ? c.x : c.y, k & 1, p, bias);
+      x[2 * k] = f.x;
+      x[2 * k + 1] = f.y;
     }
   }
-  if (__builtin_expect(s >= 254u, 0)) {  // 128 p is past fp32, and 255 is NaN
+  if (__builtin_expect(s >= 250u, 0)) {  // 1,152 p is past fp32, and 255 is NaN
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
       if (FMT == DSR_MX_INT8)
@@ -172,7 +183,7 @@ __device__ __forceinline__ void mx_decode(uint2 c, uint32_t s, float* x) {
 // Scale codes above it may read as more than the type holds, and 255 as NaN.
 template <int FMT, int DT>
 __device__ __forceinline__ constexpr uint32_t top_scale() {
-  return DT == DSR_DTYPE_BF16 ? (FMT == DSR_MX_FP4 ? 252u : 253u)
+  return DT == DSR_DTYPE_BF16 ? (FMT == DSR_MX_FP4 ? 252u : 249u)
                               : (FMT == DSR_MX_FP4 ? 140u : 141u);
 }
 
@@ -187,8 +198,7 @@ __device__ __forceinline__ uint32_t pack2(float x, float y) {
 }
 
 // 8 codes under scale code s as 8 values of the type; above top_scale()
-// dequantise_any(). e2m1 has an instruction for it; int8 goes through unsigned bytes, whose
-// conversion is a plain one: (u - 128) 2^e is one fused step, exact.
+// dequantise_any(). e2m1 has an instruction for it.
 template <int FMT, int DT>
 __device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
   u32x4 o;
@@ -206,16 +216,11 @@ __device__ __forceinline__ u32x4 dequantise(const uint32_t* w, uint32_t s) {
     DSR_DQ(3)
 #undef DSR_DQ
   } else {
-    const float e = __builtin_ldexpf(1.0f, (int)s - 133), bias = -128.0f * e;
+    const float p = __builtin_ldexpf(1.0f, (int)s - 133), bias = -1152.0f * p;
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint32_t u = w[h] ^ 0x80808080u;
-      const float x0 = __builtin_fmaf((float)(u & 255u), e, bias);
-      const float x1 = __builtin_fmaf((float)(u >> 8 & 255u), e, bias);
-      const float x2 = __builtin_fmaf((float)(u >> 16 & 255u), e, bias);
-      const float x3 = __builtin_fmaf((float)(u >> 24), e, bias);
-      o[2 * h] = pack2<DT>(x0, x1);
-      o[2 * h + 1] = pack2<DT>(x2, x3);
+    for (int k = 0; k < 4; ++k) {
+      const f32x2 x = int8_pair(w[k >> 1], k & 1, p, bias);
+      o[k] = pack2<DT>(x.x, x.y);
     }
   }
   return o;
