@@ -42,6 +42,7 @@ struct MxArgs {
   int32_t vecs;           // 16-byte vectors (8 elements) of a page
   int32_t codes, scales;  // section bytes of one half
   int32_t heads, block;
+  int32_t block_shift;    // log2 of block, or -1
   FastDiv row_vecs, by_block, by_heads;  // vectors per row; block; heads
 };
 
@@ -561,7 +562,16 @@ __device__ __forceinline__ bool mx_token(const MxArgs& a, const int64_t* slots,
   o->c = (int)(v - (uint32_t)h * a.row_vecs.d);
   const int64_t slot = slots[t], row = rows[t];
   if (slot < 0 || row < 0) return false;
-  const int64_t blk = slot / a.block, off = row / a.block;
+  // a 64-bit division is some hundred instructions (67,000 tokens of Qwen2-0.5B loaded by
+  // slot 289 -> 230 us, saved 277 -> 271)
+  int64_t blk, off;
+  if (a.block_shift >= 0) {
+    blk = slot >> a.block_shift;
+    off = row >> a.block_shift;
+  } else {
+    blk = slot / a.block;
+    off = row / a.block;
+  }
   const int ct = (int)(slot - blk * a.block), rt = (int)(row - off * a.block);
   if (blk >= a.num_blocks || (off & 15)) return false;
   const int64_t at = off + (int64_t)(a.layer0 + l) * a.layer_bytes;

@@ -44,6 +44,7 @@ int mx_args(const dsr_mx_args* in, int first, int count, const void* t1, const v
   a->scales = (int)scales;
   a->heads = in->num_heads;
   a->block = in->block_size;
+  a->block_shift = in->block_size & (in->block_size - 1) ? -1 : __builtin_ctz((unsigned)in->block_size);
   a->row_vecs = fast_div((uint32_t)in->head_dim / 8);
   a->by_block = fast_div((uint32_t)in->block_size);
   a->by_heads = fast_div((uint32_t)in->num_heads);
