@@ -273,7 +273,6 @@ __device__ __forceinline__ void phase() { __builtin_amdgcn_sched_barrier(0); }
 constexpr int kAttendWaves = 4;
 constexpr int kStep = 32;  // tokens of a step
 
-
 // Bytes of a V row in LDS: 32 more than it holds, so that 8 rows of two 16-byte chunks (a
 // transposing read of 32 lanes) and 8 rows of one (a write of 8 lanes) meet each bank once,
 // and every address is a lane's base and a constant.
@@ -282,7 +281,10 @@ __device__ __forceinline__ constexpr int lds_row() {
   return 2 * D + 32;
 }
 
-// Waves per SIMD that the registers are to leave room for.
+// Waves per SIMD that the registers are to leave room for. Decode batch (e2m1, head_dim
+// 128) at 2, 3 and 4: 174, 177 and 179 us before the grid was made odd; a moved chunk's
+// queries spill 20 to 40 registers at 3, beside 2 waves' 106 us for questions (98 and 83
+// with fewer spills). What bounds the decode batch is its 1 KiB reads, 131 us by themselves.
 template <int D, int NQ, bool ROPE>
 constexpr int attend_waves() {
   if (NQ == 1) return D <= 64 ? 4 : D <= 128 ? 3 : 2;

@@ -11,10 +11,16 @@ namespace {
 
 constexpr int kMaxGridZ = 65535;
 
-constexpr int kAttendWgs = 2048;      // workgroups that fill the chip
-constexpr int kAttendWideWgs = 512;  // of several tiles of rows: two to a CU
+// Workgroups that the splits aim at. One tile of rows: 2,048, some eight for each CU, so that
+// ragged requests even out (decode batch of 64 x 8 heads: 1,536 150 us, 2,048 133, 3,072 142,
+// 4,096 155). Several tiles: 512, which the chip holds at once (questions 512 79 us, 256 102,
+// 1,024 96: each workgroup turns the queries and joins 32 rows).
+constexpr int kAttendWgs = 2048, kAttendWideWgs = 512;
+// Steps of heads and tokens from which a wave takes a head of its own: with as many waves as
+// the chip holds, 16 tokens' worth of 64 steps each. Below, the waves of a workgroup share a
+// head's tokens and join in LDS, which leaves the second kernel a quarter of the parts.
 constexpr int64_t kAttendLarge = 256 * 16 * 64;
-constexpr int kAttendMinChunk = 128;  // tokens: a step of each wave
+constexpr int kAttendMinChunk = 128;  // tokens of a split: a step of each wave
 
 // Tiles of 16 rows per workgroup: what is dequantised serves them all, and their
 // accumulators leave room for two waves a SIMD. 4 x 64 queries over 4,096 tokens, 2 -> 4 tiles:
