@@ -83,6 +83,25 @@ def test_token_tables_keep_the_last(seed):
         assert t.tolist() == [ridx[i] for i in want]
 
 
+@pytest.mark.parametrize("seed", range(4))
+def test_many_token_runs(seed):
+    """Enough runs for the ordering by digits, far apart, with and without repeats."""
+    rng = np.random.default_rng(seed)
+    bs, n = 16, 700
+    blocks = rng.permutation(4000)[:n] if seed < 2 else rng.integers(0, 300, n)
+    offs = rng.permutation(1 << 20)[:n] * 16 if seed % 2 else rng.integers(0, 500, n) * 16
+    part = rng.integers(1, bs + 1, n)
+    slots = np.concatenate([b * bs + np.arange(p) for b, p in zip(blocks, part)])
+    rows = np.concatenate([o * bs + np.arange(p) for o, p in zip(offs, part)])
+    for mode in (0, 1):
+        last = {}
+        for i, k in enumerate(rows if mode else slots):
+            last[int(k)] = i
+        want = [last[k] for k in sorted(last)]
+        s, r, _ = plan(slots, rows, bs, mode, blocks=4000, staging=1 << 25)
+        assert np.array_equal(s, slots[want]) and np.array_equal(r, rows[want])
+
+
 def test_token_table_refusals():
     ok = plan([3], [16 * 16 + 2], 16, 0)
     assert ok[0].tolist() == [3]
