@@ -292,7 +292,8 @@ constexpr int attend_waves() {
 }
 
 template <int FMT, int DT, int D, int NQ, bool ROPE>
-__global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx_attend_kernel(AttendArgs g) {
+__global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx_attend_kernel(
+    AttendArgs g) {
   const dsr_attend_args& a = g.a;
   constexpr int B = D / 32, NT = D / 16;
   using Tile = AttendTile<FMT, D>;
@@ -312,10 +313,12 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
   const int64_t rows = rq.q1 > rq.q0 ? (int64_t)(rq.q1 - rq.q0) * g.group : 0;
   const float ninf = -__builtin_inff();
   auto out_row = [&](int64_t row, int head) {
-    return (int64_t)(rq.q0 + (int)(row / g.group)) * a.q_heads + head * g.group + (int)(row % g.group);
+    return (int64_t)(rq.q0 + (int)(row / g.group)) * a.q_heads + head * g.group +
+           (int)(row % g.group);
   };
 
-  for (int64_t row0 = (int64_t)tile0 * (16 * NQ); row0 < rows; row0 += (int64_t)g.tiles * (16 * NQ)) {
+  for (int64_t row0 = (int64_t)tile0 * (16 * NQ); row0 < rows;
+       row0 += (int64_t)g.tiles * (16 * NQ)) {
     // this lane's columns
     int lim[NQ];
     const uint8_t* qrow[NQ];
@@ -558,6 +561,7 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
         phase();
       }
 
+      wave_lds();
       // O^T: lanes' columns 4 c ... of rows 4 quarter + r, transposed in 16-lane groups
 #pragma unroll
       for (int k = 0; k < NT; ++k) {
@@ -572,6 +576,7 @@ __global__ __launch_bounds__(kThreads, (attend_waves<D, NQ, ROPE>())) void kv_mx
 #pragma unroll
         for (int j = 0; j < NQ; ++j) acc[j][k] = mfma32<DT>(vt.v, pf[j], acc[j][k]);
       }
+      wave_lds();
 
       if (__builtin_expect(odd, 0)) {
         const float nan = __uint_as_float(0x7fc00000u);

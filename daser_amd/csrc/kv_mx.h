@@ -46,7 +46,15 @@ struct MxArgs {
   FastDiv row_vecs, by_block, by_heads;  // vectors per row; block; heads
 };
 
-// A cache row's place in the record ([H][block]) and the other way round.
+// Between a wave's writes to its part of the LDS and other lanes' reads, and before it is
+// written again. The hardware keeps a wave's LDS operations in order; this is for the compiler.
+__device__ __forceinline__ void wave_lds() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// The rotation of a load's K.
 struct MxRope {
   const float2* cos_sin;
   const int32_t* rope_idx;  // null: nothing is rotated
@@ -446,16 +454,19 @@ __global__ __launch_bounds__(kThreads) void kv_mx_gather_kernel(MxArgs a, const 
       else reinterpret_cast<uint2*>(mine)[i] = q;
       if ((lane & 3) == 0) mine[U * kWave * CB + (i >> 2)] = (uint8_t)s;
     }
+    wave_lds();
     const MxHalf o = mx_half(a, u.rec, half);
     const rsrc_t codes = make_rsrc(o.codes + (int64_t)first * CB, (int64_t)left * CB);
     const rsrc_t scales = make_rsrc(o.scales + first / 4, left / 4);
 #pragma unroll
     for (int k = 0; k < (U * CB + 15) / 16; ++k) {
       const int i = k * kWave + lane;
-      if (i * 16 < U * kWave * CB) bstore_as<POLICY>(codes, i * 16, reinterpret_cast<u32x4*>(mine)[i]);
+      if (i * 16 < U * kWave * CB)
+        bstore_as<POLICY>(codes, i * 16, reinterpret_cast<u32x4*>(mine)[i]);
     }
     if (lane < U * 16)
       __builtin_amdgcn_raw_buffer_store_b8(mine[U * kWave * CB + lane], scales, lane, 0, POLICY);
+    wave_lds();  // before the other half's
   }
 }
 
@@ -477,7 +488,8 @@ __global__ __launch_bounds__(kThreads) void kv_mx_scatter_kernel(MxArgs a, MxRop
     const int h = row - t * a.heads;
     rv = (h * a.block + t) * (int)a.row_vecs.d + c;
   }
-  const rsrc_t ck = make_rsrc(u.cache, a.page_bytes), cw = make_rsrc(u.cache + a.kv_stride, a.page_bytes);
+  const rsrc_t ck = make_rsrc(u.cache, a.page_bytes);
+  const rsrc_t cw = make_rsrc(u.cache + a.kv_stride, a.page_bytes);
   // the loads go out before the page's table is known
   const MxVec v = mx_load_vec<FMT>(mx_half(a, u.rec, 1), rv, -1);
   const MxVec w = mx_load_vec<FMT>(mx_half(a, u.rec, 0), rv, mx_partner<STYLE>(r, rv, c));
@@ -512,7 +524,8 @@ __global__ __launch_bounds__(kThreads) void kv_mx_scatter_pairs_kernel(MxArgs a,
   v[0] = mx_load_vec<FMT>(hw, rec_row * nv + c, -1);
   v[1] = mx_load_vec<FMT>(hw, rec_row * nv + c + hv, -1);
   const float2* cs = mx_table(r, u.page, u.layer);
-  const rsrc_t ck = make_rsrc(u.cache, a.page_bytes), cw = make_rsrc(u.cache + a.kv_stride, a.page_bytes);
+  const rsrc_t ck = make_rsrc(u.cache, a.page_bytes);
+  const rsrc_t cw = make_rsrc(u.cache + a.kv_stride, a.page_bytes);
   const int off = (row * nv + c) << 4;
   u32x4 lower, upper;
   if (cs) {
