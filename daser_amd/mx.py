@@ -434,7 +434,8 @@ def attend(q: torch.Tensor, fmt: MXFormat, staging: torch.Tensor, q_start, page_
     ``max_queries`` / ``max_context`` are the largest request's, for the launch's
     shape; None: from host tables, or bounds that hold for any. Results are right
     whatever they say; how the tokens are split, and so the last bit of a sum, follows
-    them. Rows of ``out`` that belong to no request are left as they were."""
+    them. Rows of ``out`` that belong to no request are left as they were, and their
+    lse is not set."""
     if q.dim() != 3 or q.dtype not in _DTYPES:
         raise ValueError("q must be bfloat16 or float16 [n, q_heads, head_dim]")
     n, heads, dim = q.shape
